@@ -471,16 +471,13 @@ int fsx_open(fsx_ctx **out, const fsx_config *cfg) {
     c->tr_slots = admit ? k.max_batch : 0;
     c->id_slots = admit ? std::max<uint64_t>(c->slots, next_pow2(std::max<uint64_t>(1024, 2 * k.max_batch))) : c->slots;
     auto fail = [&](int r) { fsx_close(c); return r; };
-    // stream priorities (A/B: FSX_STREAM_PRIO="own,aux,walk", lower = more urgent): the
-    // context stream (parse, sort) first, so a pipelined batch's short sort scans find CU
-    // slots among the previous batch's tail (-0.6 % per step, profiles/r03/ab_prio/)
-    int prio[3] = {-1, 0, 0};
-    if (const char *ps = getenv("FSX_STREAM_PRIO")) sscanf(ps, "%d,%d,%d", &prio[0], &prio[1], &prio[2]);
-    if (hipStreamCreateWithPriority(&c->own_stream, hipStreamNonBlocking, prio[0]) != hipSuccess) return fail(-EIO);
-    if (hipStreamCreateWithPriority(&c->aux_stream, hipStreamNonBlocking, prio[1]) != hipSuccess) return fail(-EIO);
+    // all at the default priority: work on streams of different priorities can stall for good
+    // on this platform (an urgent context stream was worth 0.6 % of a step)
+    if (hipStreamCreateWithFlags(&c->own_stream, hipStreamNonBlocking) != hipSuccess) return fail(-EIO);
+    if (hipStreamCreateWithFlags(&c->aux_stream, hipStreamNonBlocking) != hipSuccess) return fail(-EIO);
     if (hipEventCreateWithFlags(&c->fork_ev, hipEventDisableTiming) != hipSuccess) return fail(-EIO);
     if (hipEventCreateWithFlags(&c->join_ev, hipEventDisableTiming) != hipSuccess) return fail(-EIO);
-    if (hipStreamCreateWithPriority(&c->walk_stream, hipStreamNonBlocking, prio[2]) != hipSuccess) return fail(-EIO);
+    if (hipStreamCreateWithFlags(&c->walk_stream, hipStreamNonBlocking) != hipSuccess) return fail(-EIO);
     if (hipEventCreateWithFlags(&c->walk_fork_ev, hipEventDisableTiming) != hipSuccess) return fail(-EIO);
     if (hipEventCreateWithFlags(&c->walk_join_ev, hipEventDisableTiming) != hipSuccess) return fail(-EIO);
     if (hipEventCreateWithFlags(&c->heavy_fork_ev, hipEventDisableTiming) != hipSuccess) return fail(-EIO);

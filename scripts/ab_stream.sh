@@ -1,6 +1,6 @@
 #!/bin/bash
 # A/B of run-time switches on the headline stream (pipelined) and its unpipelined twin:
-#   scripts/ab_stream.sh "" "FSX_STREAM_PRIO=-1,0,0" ...
+#   scripts/ab_stream.sh "" "FSX_TAIL_AT=1" ...
 cd "${GRAFT_REPO_ROOT:-$(dirname "$0")/..}"
 mkdir -p gpurun_out
 k=0
