@@ -33,11 +33,11 @@ COMMON = [
 LIBS = {
     "libfsx_hip.so": ["fsx_device.hip", "fsx_limiters.hip", "fsx_shard.hip", "fsx_pcap.hip",
                       "fsx_flows.hip", "fsx_score.hip", "fsx_heavy.hip",
-                      "fsx_api.hip"],
+                      "fsx_linear.hip", "fsx_logprobs.hip", "fsx_api.hip"],
     "libfsx_synth.so": ["fsx_synth.hip"],
 }
 HEADERS = ["fsx_internal.h", "fsx_synth_common.h", "fsx_dev_common.h", "fsx_q8.h", "fsx_seg.h", "fsx_shard.h", "fsx_walk.h",
-           "fsx_flow_common.h", "fsx_heavy_view.h", "fsx_search.h", "fsx_plan.h"]
+           "fsx_flow_common.h", "fsx_heavy_view.h", "fsx_search.h", "fsx_plan.h", "fsx_head.h"]
 
 
 def _stale(out: Path, srcs: list[Path]) -> bool:

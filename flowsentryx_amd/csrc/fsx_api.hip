@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "../../include/fsx_hip.h"
+#include "fsx_head.h"
 #include "fsx_internal.h"
 #include "fsx_shard.h"
 
@@ -1698,6 +1699,125 @@ int fsx_score(fsx_ctx *c, const float *feat, size_t n, float *prob, uint8_t *mal
     HIPCHK(c, hipMemcpyAsync(prob, c->d_prob, n * 4, hipMemcpyDeviceToHost, c->stream));
     HIPCHK(c, hipMemcpyAsync(mal, c->d_dec, n, hipMemcpyDeviceToHost, c->stream));
     HIPCHK(c, hipStreamSynchronize(c->stream));
+    return 0;
+}
+
+// ---- heads of free size (fsx_linear.hip, fsx_logprobs.hip)
+
+static bool float_type(int dtype) {
+    return dtype == FSX_DTYPE_F32 || dtype == FSX_DTYPE_F16 || dtype == FSX_DTYPE_BF16;
+}
+
+// A matrix in device memory: pointer, rows that do not overlap, an extent that can exist.
+static int check_matrix(fsx_ctx *c, const char *what, const void *p, uint32_t size, uint64_t rows, uint64_t cols,
+                        uint64_t ld) {
+    if (rows > kMaxRows || ld > kMaxBytes / (rows * size)) return set_err(c, -EINVAL, "%s: size out of range", what);
+    if (ld < cols)
+        return set_err(c, -EINVAL, "%s: rows of %llu elements are %llu apart", what, (unsigned long long)cols,
+                       (unsigned long long)ld);
+    if (!p) return set_err(c, -EINVAL, "%s: null buffer", what);
+    if ((uintptr_t)p % size) return set_err(c, -EINVAL, "%s: misaligned buffer", what);
+    return 0;
+}
+
+static int check_work(fsx_ctx *c, const void *d_work, size_t work_bytes, uint64_t need) {
+    if (work_bytes < need)
+        return set_err(c, -EINVAL, "workspace of %zu bytes, %llu needed", work_bytes, (unsigned long long)need);
+    if (need && (!d_work || (uintptr_t)d_work % 16)) return set_err(c, -EINVAL, "null or misaligned workspace");
+    return 0;
+}
+
+int fsx_quantize_rows_device(fsx_ctx *c, const void *d_x, int x_dtype, size_t rows, size_t cols, size_t ldx,
+                             int8_t *d_codes, size_t ld_codes, float *d_scale) {
+    if (!c) return -EINVAL;
+    if (!float_type(x_dtype)) return set_err(c, -EINVAL, "rows of type %d: F32, F16 or BF16", x_dtype);
+    if (cols < 1 || cols > kMaxDim) return set_err(c, -EINVAL, "rows of %zu elements", cols);
+    if (rows == 0) return 0;
+    int rc = check_matrix(c, "x", d_x, elem_size(x_dtype), rows, cols, ldx);
+    if (!rc) rc = check_matrix(c, "codes", d_codes, 1, rows, cols, ld_codes);
+    if (!rc) rc = check_matrix(c, "scales", d_scale, 4, rows, 1, 1);
+    if (!rc) rc = sel(c);
+    if (rc) return rc;
+    const hipError_t e = launch_quantize_rows(d_x, x_dtype, rows, (uint32_t)cols, ldx, d_codes, ld_codes, d_scale,
+                                              c->stream);
+    if (e != hipSuccess) return set_err(c, -EIO, "quantize launch: %s", hipGetErrorString(e));
+    return 0;
+}
+
+static bool layer_sizes_ok(const fsx_q8_linear *l) {
+    return l && l->in_features >= 1 && l->in_features <= kMaxIn && l->out_features <= kMaxDim;
+}
+
+size_t fsx_linear_q8_work(const fsx_q8_linear *layer, int x_dtype, size_t rows) {
+    if (!layer_sizes_ok(layer) || rows == 0 || rows > kMaxRows || layer->out_features == 0) return 0;
+    if (x_dtype != FSX_DTYPE_I8 && !float_type(x_dtype)) return 0;
+    return linear_work(rows, (uint32_t)layer->in_features, (uint32_t)layer->out_features, x_dtype);
+}
+
+int fsx_linear_q8_device(fsx_ctx *c, const fsx_q8_linear *layer, const void *d_x, int x_dtype, size_t ldx,
+                         const float *d_x_scale, size_t rows, void *d_y, int y_dtype, size_t ldy, void *d_work,
+                         size_t work_bytes) {
+    if (!c) return -EINVAL;
+    if (!layer) return set_err(c, -EINVAL, "null layer");
+    if (!layer_sizes_ok(layer))
+        return set_err(c, -EINVAL, "a layer of %llu to %llu features", (unsigned long long)layer->in_features,
+                       (unsigned long long)layer->out_features);
+    if (layer->activation < FSX_ACT_NONE || layer->activation > FSX_ACT_SIGMOID || layer->reserved)
+        return set_err(c, -EINVAL, "unknown activation %d", layer->activation);
+    if (x_dtype != FSX_DTYPE_I8 && !float_type(x_dtype)) return set_err(c, -EINVAL, "x of type %d", x_dtype);
+    if (!float_type(y_dtype)) return set_err(c, -EINVAL, "y of type %d: F32, F16 or BF16", y_dtype);
+    const uint64_t k = layer->in_features, n = layer->out_features;
+    if (rows == 0 || n == 0) return 0;
+    int rc = check_matrix(c, "x", d_x, elem_size(x_dtype), rows, k, ldx);
+    if (!rc) rc = check_matrix(c, "weight", layer->weight, 1, n, k, layer->ld_weight);
+    if (!rc) rc = check_matrix(c, "weight scales", layer->weight_scale, 4, n, 1, 1);
+    if (!rc && layer->bias) rc = check_matrix(c, "bias", layer->bias, 4, n, 1, 1);
+    if (!rc && x_dtype == FSX_DTYPE_I8) rc = check_matrix(c, "x scales", d_x_scale, 4, rows, 1, 1);
+    if (!rc && x_dtype != FSX_DTYPE_I8 && d_x_scale) rc = set_err(c, -EINVAL, "x scales given for float rows");
+    if (!rc) rc = check_matrix(c, "y", d_y, elem_size(y_dtype), rows, n, ldy);
+    if (!rc) rc = check_work(c, d_work, work_bytes, linear_work(rows, (uint32_t)k, (uint32_t)n, x_dtype));
+    if (!rc) rc = sel(c);
+    if (rc) return rc;
+    LinearArgs a{};
+    a.x = d_x; a.x_scale = d_x_scale; a.ldx = ldx;
+    a.w = layer->weight; a.w_scale = layer->weight_scale; a.bias = layer->bias; a.ldw = layer->ld_weight;
+    a.rows = rows; a.k = (uint32_t)k; a.n = (uint32_t)n; a.act = layer->activation;
+    a.y = d_y; a.ldy = ldy;
+    const hipError_t e = launch_linear(a, x_dtype, y_dtype, d_work, c->stream);
+    if (e != hipSuccess) return set_err(c, -EIO, "linear launch: %s", hipGetErrorString(e));
+    return 0;
+}
+
+size_t fsx_logprobs_work(size_t rows, size_t classes, uint32_t top_k) {
+    if (rows == 0 || rows > kMaxRows || classes < 1 || classes > kMaxDim || top_k > FSX_TOP_MAX) return 0;
+    return logprobs_work(rows, (uint32_t)classes, top_k);
+}
+
+int fsx_logprobs_device(fsx_ctx *c, const void *d_logits, int dtype, size_t rows, size_t classes, size_t ld,
+                        const int32_t *d_target, float *d_logprob, float *d_entropy, uint32_t top_k,
+                        int32_t *d_top_id, float *d_top_logprob, void *d_work, size_t work_bytes) {
+    if (!c) return -EINVAL;
+    if (!float_type(dtype)) return set_err(c, -EINVAL, "logits of type %d: F32, F16 or BF16", dtype);
+    if (classes < 1 || classes > kMaxDim) return set_err(c, -EINVAL, "rows of %zu classes", classes);
+    if (top_k > FSX_TOP_MAX) return set_err(c, -EINVAL, "top_k %u: at most %d", top_k, FSX_TOP_MAX);
+    if (rows == 0) return 0;
+    if (!d_target != !d_logprob) return set_err(c, -EINVAL, "targets and their log probabilities go together");
+    if (!top_k && (d_top_id || d_top_logprob)) return set_err(c, -EINVAL, "alternatives without top_k");
+    int rc = check_matrix(c, "logits", d_logits, elem_size(dtype), rows, classes, ld);
+    if (!rc && d_target) rc = check_matrix(c, "targets", d_target, 4, rows, 1, 1);
+    if (!rc && d_target) rc = check_matrix(c, "log probabilities", d_logprob, 4, rows, 1, 1);
+    if (!rc && d_entropy) rc = check_matrix(c, "entropies", d_entropy, 4, rows, 1, 1);
+    if (!rc && top_k) rc = check_matrix(c, "alternatives", d_top_id, 4, rows, top_k, top_k);
+    if (!rc && top_k) rc = check_matrix(c, "alternatives' log probabilities", d_top_logprob, 4, rows, top_k, top_k);
+    if (!rc) rc = check_work(c, d_work, work_bytes, logprobs_work(rows, (uint32_t)classes, top_k));
+    if (!rc) rc = sel(c);
+    if (rc) return rc;
+    LogprobArgs a{};
+    a.x = d_logits; a.rows = rows; a.ld = ld; a.v = (uint32_t)classes; a.top = top_k;
+    a.target = d_target; a.logprob = d_logprob; a.entropy = d_entropy;
+    a.top_id = d_top_id; a.top_lp = d_top_logprob; a.work = d_work;
+    const hipError_t e = launch_logprobs(a, dtype, c->stream);
+    if (e != hipSuccess) return set_err(c, -EIO, "logprobs launch: %s", hipGetErrorString(e));
     return 0;
 }
 

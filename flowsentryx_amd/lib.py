@@ -57,6 +57,11 @@ LIMIT_FIXED_WINDOW = 0
 LIMIT_SLIDING_WINDOW = 1
 LIMIT_TOKEN_BUCKET = 2
 
+# element types and activations of the free-size heads
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_I8 = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_SIGMOID = 0, 1, 2
+TOP_MAX = 64
+
 
 class FsxError(RuntimeError):
     def __init__(self, code: int, msg: str):
@@ -95,6 +100,19 @@ class FsxQ8Model(C.Structure):
         ("in_zero_point", C.c_int32),
         ("out_scale", C.c_float),
         ("out_zero_point", C.c_int32),
+    ]
+
+
+class FsxQ8Linear(C.Structure):
+    _fields_ = [
+        ("weight", C.c_void_p),
+        ("weight_scale", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("in_features", C.c_uint64),
+        ("out_features", C.c_uint64),
+        ("ld_weight", C.c_uint64),
+        ("activation", C.c_int32),
+        ("reserved", C.c_uint32),
     ]
 
 
@@ -144,6 +162,12 @@ def load_library() -> C.CDLL:
         "fsx_load_q8_model": (C.c_int, [vp, C.POINTER(FsxQ8Model)]),
         "fsx_score": (C.c_int, [vp, vp, sz, vp, vp]),
         "fsx_score_device": (C.c_int, [vp, vp, sz, vp, vp]),
+        "fsx_quantize_rows_device": (C.c_int, [vp, vp, C.c_int, sz, sz, sz, vp, sz, vp]),
+        "fsx_linear_q8_work": (sz, [C.POINTER(FsxQ8Linear), C.c_int, sz]),
+        "fsx_linear_q8_device": (C.c_int, [vp, C.POINTER(FsxQ8Linear), vp, C.c_int, sz, vp, sz, vp, C.c_int, sz,
+                                           vp, sz]),
+        "fsx_logprobs_work": (sz, [sz, sz, C.c_uint32]),
+        "fsx_logprobs_device": (C.c_int, [vp, vp, C.c_int, sz, sz, sz, vp, vp, vp, C.c_uint32, vp, vp, vp, sz]),
         "fsx_flow_features": (C.c_int, [vp, vp, vp, vp, sz, sz, vp, vp, vp, C.POINTER(sz)]),
         "fsx_flows_begin": (C.c_int, [vp]),
         "fsx_flows_end": (C.c_int, [vp, vp, vp, vp, vp, vp, sz, vp]),
@@ -183,7 +207,8 @@ ABI_SYMBOLS = [
     "fsx_process_batch_device", "fsx_verdict_records_device", "fsx_process_records_device",
     "fsx_map_lookup", "fsx_map_update", "fsx_map_update_batch", "fsx_map_delete", "fsx_map_dump",
     "fsx_get_stats",
-    "fsx_reset", "fsx_load_q8_model", "fsx_score", "fsx_score_device", "fsx_flow_features",
+    "fsx_reset", "fsx_load_q8_model", "fsx_score", "fsx_score_device", "fsx_quantize_rows_device",
+    "fsx_linear_q8_work", "fsx_linear_q8_device", "fsx_logprobs_work", "fsx_logprobs_device", "fsx_flow_features",
     "fsx_flows_begin", "fsx_flows_end", "fsx_flow_partials_records_device", "fsx_flows_merge_device",
     "fsx_flows_merge_counted_device", "fsx_shard_pack_filtered_device", "fsx_shard_filter_plan_device",
     "fsx_blocklist_replica_blocks_device",
@@ -209,6 +234,25 @@ def shard_owner(key16: bytes, family: int, n_shards: int) -> int:
     """Owner rank of a source (include/fsx_hip.h fsx_shard_owner; host-only)."""
     k = bytes(key16).ljust(16, b"\0")
     return int(load_library().fsx_shard_owner(k, int(family), int(n_shards)))
+
+
+def q8_linear(d_weight: int, d_weight_scale: int, d_bias: int | None, in_features: int, out_features: int,
+              ld_weight: int | None = None, activation: int = ACT_NONE) -> FsxQ8Linear:
+    """An int8 layer over device memory (include/fsx_hip.h fsx_q8_linear): codes
+    [out_features][ld_weight], a scale for every output channel, optional bias. The caller keeps
+    the buffers."""
+    return FsxQ8Linear(d_weight or None, d_weight_scale or None, d_bias or None, in_features, out_features,
+                       in_features if ld_weight is None else ld_weight, activation, 0)
+
+
+def linear_q8_work(layer: FsxQ8Linear, x_dtype: int, rows: int) -> int:
+    """Workspace bytes of FsxContext.linear_q8_device for `rows` rows (0: none; host only)."""
+    return int(load_library().fsx_linear_q8_work(C.byref(layer), x_dtype, rows))
+
+
+def logprobs_work(rows: int, classes: int, top_k: int) -> int:
+    """Workspace bytes of FsxContext.logprobs_device (0: none; host only)."""
+    return int(load_library().fsx_logprobs_work(rows, classes, top_k))
 
 
 def default_config(**overrides) -> FsxConfig:
@@ -481,6 +525,34 @@ class FsxContext:
 
     def score_device(self, d_feat: int, n: int, d_prob: int, d_dec: int):
         self._check(self._lib.fsx_score_device(self._h, d_feat, n, d_prob, d_dec), "fsx_score_device")
+
+    # -- heads of free size (device pointers, asynchronous on the context stream)
+    def quantize_rows_device(self, d_x: int, x_dtype: int, rows: int, cols: int, ldx: int, d_codes: int,
+                             ld_codes: int, d_scale: int):
+        """int8 codes of every row of floats and one scale a row (include/fsx_hip.h
+        fsx_quantize_rows_device)."""
+        self._check(self._lib.fsx_quantize_rows_device(self._h, d_x, x_dtype, rows, cols, ldx, d_codes, ld_codes,
+                                                       d_scale), "fsx_quantize_rows_device")
+
+    def linear_q8_device(self, layer: FsxQ8Linear, d_x: int, x_dtype: int, ldx: int, d_x_scale: int | None,
+                         rows: int, d_y: int, y_dtype: int, ldy: int, d_work: int | None = None,
+                         work_bytes: int = 0):
+        """y = act(x . weight^T with a scale for every row and channel + bias): x as int8 codes with
+        d_x_scale, or as floats that the call quantises by row (d_x_scale None); a workspace of
+        linear_q8_work bytes."""
+        self._check(self._lib.fsx_linear_q8_device(self._h, C.byref(layer), d_x, x_dtype, ldx, d_x_scale or None,
+                                                   rows, d_y, y_dtype, ldy, d_work or None, work_bytes),
+                    "fsx_linear_q8_device")
+
+    def logprobs_device(self, d_logits: int, dtype: int, rows: int, classes: int, ld: int, d_target: int | None,
+                        d_logprob: int | None, d_entropy: int | None, top_k: int = 0, d_top_id: int | None = None,
+                        d_top_logprob: int | None = None, d_work: int | None = None, work_bytes: int = 0):
+        """Of every row of logits: the log probability of a given class, the entropy and the top_k
+        most probable classes; a workspace of logprobs_work bytes."""
+        self._check(self._lib.fsx_logprobs_device(self._h, d_logits, dtype, rows, classes, ld, d_target or None,
+                                                  d_logprob or None, d_entropy or None, top_k, d_top_id or None,
+                                                  d_top_logprob or None, d_work or None, work_bytes),
+                    "fsx_logprobs_device")
 
     def flow_features(self, hdr: np.ndarray, length: np.ndarray, ts: np.ndarray):
         hdr = np.ascontiguousarray(hdr, dtype=np.uint8).reshape(-1, HDR_BYTES)

@@ -296,6 +296,79 @@ int fsx_score(fsx_ctx *ctx, const float *features, size_t n, float *prob,
 int fsx_score_device(fsx_ctx *ctx, const float *d_features, size_t n, float *d_prob,
                      uint8_t *d_malicious);
 
+/* ---- Heads of free size: int8 layers and the answers of a head of several classes.
+ * fsx_score is the reference's Linear(8, 1) with its per-tensor scales (model/model.py:132-137);
+ * these three are for any other head (build-defined, parity unpinned: the reference has none).
+ *
+ * All buffers are device memory of the context's GPU, rows are `ld` elements apart (ld >= the
+ * row's length; a row's end up to ld is neither read as data nor written), and outputs do not
+ * overlap inputs, each other or the workspace. The calls are asynchronous on the context
+ * stream and keep nothing: no device memory is allocated, nothing is cached between calls, so
+ * they may be captured into a HIP graph (a workspace is then the graph's own: one that two
+ * graphs share is overwritten when both run at once). With 0 rows nothing is launched.
+ * Results do not depend on timing: the same call gives the same bits.
+ *
+ * Errors: -EINVAL (with fsx_last_error) for an unknown type, a null or misaligned pointer
+ * (elements at their size, the workspace at 16 bytes), ld below the row's length, a size out
+ * of range, or a workspace below the size that the *_work function gives. */
+#define FSX_DTYPE_F32 0
+#define FSX_DTYPE_F16 1
+#define FSX_DTYPE_BF16 2
+#define FSX_DTYPE_I8 3
+
+/* int8 codes of every row of floats (F32 / F16 / BF16), with one scale a row:
+ *   scale = max(amax / 127 rounded to 32 bits, 2^-126),  amax = the row's largest |x|
+ *   code  = x / scale to the nearest whole number, halves to even (exact: as if in infinite
+ *           precision with that scale); |code| <= 127
+ * A row that holds a NaN or an infinity gets codes 0 and the scale NaN, so that a product
+ * over it is NaN. Weights by output channel are quantised the same way, a channel a row.
+ * 1 <= cols < 2^31. */
+int fsx_quantize_rows_device(fsx_ctx *ctx, const void *d_x, int x_dtype, size_t rows, size_t cols, size_t ldx,
+                             int8_t *d_codes, size_t ld_codes, float *d_scale);
+
+/* y[r][n] = act((float)(sum over k of x[r][k] * weight[n][k]) * x_scale[r] * weight_scale[n] + bias[n])
+ * rounded once to y's type; the sum is exact (int32). RELU keeps NaN; SIGMOID is
+ * 1 / (1 + e^-v). x is either codes (FSX_DTYPE_I8) with their row scales d_x_scale, or floats
+ * (d_x_scale NULL) whose rows are quantised within the call as fsx_quantize_rows_device does.
+ * 1 <= in_features <= 131071 (the sum of any int8 codes then fits in 32 bits). */
+#define FSX_ACT_NONE 0
+#define FSX_ACT_RELU 1
+#define FSX_ACT_SIGMOID 2
+typedef struct fsx_q8_linear {
+    const int8_t *weight;        /* device, [out_features][ld_weight] codes */
+    const float *weight_scale;   /* device, [out_features] */
+    const float *bias;           /* device, [out_features], or NULL */
+    uint64_t in_features;
+    uint64_t out_features;       /* < 2^31 */
+    uint64_t ld_weight;
+    int32_t activation;          /* FSX_ACT_* */
+    uint32_t reserved;           /* 0 */
+} fsx_q8_linear;
+/* Workspace bytes of the call below (0: none needed; host only). Quantised rows live there,
+ * and the partial sums of products with few rows. 0 for arguments that the call refuses. */
+size_t fsx_linear_q8_work(const fsx_q8_linear *layer, int x_dtype, size_t rows);
+int fsx_linear_q8_device(fsx_ctx *ctx, const fsx_q8_linear *layer, const void *d_x, int x_dtype, size_t ldx,
+                         const float *d_x_scale, size_t rows, void *d_y, int y_dtype, size_t ldy,
+                         void *d_work, size_t work_bytes);
+
+/* The answers of every row of logits (F32 / F16 / BF16), under p = softmax(row):
+ *   d_logprob[r] = log p[d_target[r]]; 0 where the target is -1 (none asked for), NaN for any
+ *                  other target outside 0 .. classes - 1. Both pointers, or both NULL.
+ *   d_entropy[r] = -sum p log p (natural logarithm), or NULL
+ *   d_top_id / d_top_logprob [r][top_k]: the top_k most probable classes and their log
+ *                  probabilities, in falling order, ties by the lowest class; top_k 0: NULL
+ * A logit of -inf is a masked class: its probability is 0 and it is never an alternative;
+ * places that no class is left for hold id -1 and -inf. A row with every class masked has
+ * logprob -inf and entropy 0. In a row that holds a NaN or +inf every float is NaN (but the 0
+ * of a row without a target) and every id -1. 1 <= classes < 2^31, top_k <= FSX_TOP_MAX. */
+#define FSX_TOP_MAX 64
+/* Workspace bytes of the call below (0: none needed; host only): the partial results of
+ * long rows that are split over the GPU. */
+size_t fsx_logprobs_work(size_t rows, size_t classes, uint32_t top_k);
+int fsx_logprobs_device(fsx_ctx *ctx, const void *d_logits, int dtype, size_t rows, size_t classes, size_t ld,
+                        const int32_t *d_target, float *d_logprob, float *d_entropy, uint32_t top_k,
+                        int32_t *d_top_id, float *d_top_logprob, void *d_work, size_t work_bytes);
+
 /* One global batch's flow features delivered over several calls (the owner side of the
  * sharded path, where a source's packets arrive in sub-batches, in global arrival order):
  * after fsx_flows_begin, every fsx_process_batch_device / fsx_process_records_device call
