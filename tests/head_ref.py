@@ -36,7 +36,12 @@ def linear(codes, x_scale, weight, weight_scale, bias, act, dtype):
     elif act == "sigmoid":
         y = torch.sigmoid(y)
         tol = y * (1 - y) * (tol + 2 * U) * 1.01 + 4 * U * y
-    return y, tol * 1.01 + HALF_STEP[dtype] * 1.01 * y.abs() + TINY[dtype]
+    # half a step above the type's largest value and beyond, a rounded result is infinite
+    top = torch.finfo(dtype).max * (1 + HALF_STEP[dtype] / (2 - 2 * HALF_STEP[dtype]))
+    assert not ((y.abs() - top).abs() <= 2 * tol).any(), "inputs that leave open whether a result overflows"
+    y = torch.where(y.abs() >= top, torch.copysign(torch.full_like(y, float("inf")), y), y)
+    tol = torch.where(y.isinf(), torch.zeros_like(tol), tol)
+    return y, tol * 1.01 + HALF_STEP[dtype] * 1.01 * torch.where(y.isinf(), torch.zeros_like(y), y).abs() + TINY[dtype]
 
 
 def logprobs(x: torch.Tensor, target, top: int):

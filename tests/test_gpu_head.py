@@ -268,6 +268,27 @@ def test_linear_far_rows(head):
     head_ref.assert_close(far_y, ref, tol, "y")
 
 
+def test_linear_several_launches(head):
+    """More channels than one launch takes: each part of them has the bits of its own product."""
+    g = gen_of("slabs")
+    n, cuts = (1 << 20) * 2 + 100, [0, 70, (1 << 20) - 5, (1 << 20) + 90, (1 << 21) + 100]
+    for rows, k, xt in ((2, 8, torch.float32), (3, 70, torch.float32), (5, 70, torch.float32), (70, 66, torch.float16)):
+        w = torch.randint(-128, 128, (n, k), dtype=torch.int8, device="cuda")
+        ws = torch.rand(n, device="cuda")
+        bias = torch.randn(n, device="cuda")
+        x = rows_of(g, rows, k, 0, xt)
+        y, part = torch.empty(rows, n, dtype=torch.float16, device="cuda"), torch.empty(rows, n, dtype=torch.float16, device="cuda")
+        layer = head.layer(w, ws, bias, "relu")
+        work = head.linear_work(layer, x)
+        torch.cuda.synchronize()
+        head.linear(layer, x, None, y, work)
+        for a, b in zip(cuts, cuts[1:]):
+            head.linear(head.layer(w[a:b], ws[a:b], bias[a:b], "relu"), x, None, part[:, a:b], work)
+        torch.cuda.synchronize()
+        assert torch.equal(y, part)
+        check_linear(head, x, None, w[-300:], ws[-300:], bias[-300:], "relu", torch.float16)
+
+
 # ---------------------------------------------------------------- log probabilities
 
 def check_logprobs(head, x, target=True, entropy=True, top=5):

@@ -63,7 +63,7 @@ def lin(fake, native, work=0, work_bytes=0, **over):
     (dict(ldx=31), "apart"), (dict(ldw=31), "apart"), (dict(ldy=15), "apart"), (dict(w=None), "null"),
     (dict(ws=None), "null"), (dict(x=None), "null"), (dict(xs=None), "null"), (dict(y=None), "null"),
     (dict(bias=P + 2), "misaligned"), (dict(y=P + 2), "misaligned"), (dict(yt=1, y=P + 1), "misaligned"),
-    (dict(xt=0), "x scales given"), (dict(xt=2, xs=None), "workspace"), (dict(rows=1 << 41), "range")])
+    (dict(xt=0), "x scales given"), (dict(xt=2, xs=None, rows=200, k=500, ldx=500, ldw=500), "workspace"), (dict(rows=1 << 41), "range")])
 def test_linear_refusals(fake, native, over, word):
     refused(fake, lin(fake, native, **over), word)
 
