@@ -73,14 +73,18 @@ template <> struct Elem<FSX_DTYPE_BF16> { using T = __bf16; };
 // which the first `ok` exist; the others are `fill`.
 template <typename T, int N>
 __device__ __forceinline__ void load_row(const T *p, int64_t ok, float fill, float (&v)[N]) {
+    T t[N];
     if (ok >= N) {
-        T t[N];
         __builtin_memcpy(t, p, sizeof(t));
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = (float)t[i];
     } else {
+        // (loads without conditions, behind the end the first element again: all are under way at once)
+        if (ok > 0)
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = i < ok ? (float)p[i] : fill;
+            for (int i = 0; i < N; ++i) t[i] = p[i < ok ? i : 0];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i < ok ? (float)t[i] : fill;
     }
 }
 #endif

@@ -153,7 +153,9 @@ __device__ __forceinline__ v4i load16(const int8_t *p, int64_t ok) {
     } else if (ok > 0) {
         int8_t b[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) b[i] = i < ok ? p[i] : (int8_t)0;
+        for (int i = 0; i < 16; ++i) b[i] = p[i < ok ? i : 0];   // (no conditions: all under way at once)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) b[i] = i < ok ? b[i] : (int8_t)0;
         __builtin_memcpy(&v, b, 16);
     }
     return v;

@@ -15,6 +15,39 @@ namespace fsx {
 constexpr float kLowest = -3.402823466e38f;   // the maximum of no values: finite, so that -inf - m is -inf
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The value of lane ^ O, without LDS where the hardware has a lane permutation for it.
+template <int O> __device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
+    static_assert(O == 1 || O == 2 || O == 4 || O == 8 || O == 16 || O == 32, "one bit");
+    if constexpr (O == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);          // quad_perm 1 0 3 2
+    else if constexpr (O == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);     // quad_perm 2 3 0 1
+    else if constexpr (O == 4) return __builtin_amdgcn_ds_swizzle(v, 0x101F);                // xor 4
+    else if constexpr (O == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, true);    // row_ror 8
+    else if constexpr (O == 16) return __builtin_amdgcn_ds_swizzle(v, 0x401F);               // xor 16
+    else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return __lane_id() < 32 ? r[1] : r[0];
+    }
+}
+template <int O> __device__ __forceinline__ float xor_lane(float v) {
+    return __uint_as_float(xor_lane<O>(__float_as_uint(v)));
+}
+template <int O> __device__ __forceinline__ unsigned long long xor_lane(unsigned long long v) {
+    return (unsigned long long)xor_lane<O>((uint32_t)(v >> 32)) << 32 | xor_lane<O>((uint32_t)v);
+}
+// f over the G lanes (a power of two) of a group, in every lane of it
+template <int G, typename T, typename F> __device__ __forceinline__ T group_all(T v, F f) {
+    if constexpr (G > 1) v = f(v, xor_lane<1>(v));
+    if constexpr (G > 2) v = f(v, xor_lane<2>(v));
+    if constexpr (G > 4) v = f(v, xor_lane<4>(v));
+    if constexpr (G > 8) v = f(v, xor_lane<8>(v));
+    if constexpr (G > 16) v = f(v, xor_lane<16>(v));
+    if constexpr (G > 32) v = f(v, xor_lane<32>(v));
+    return v;
+}
+struct Larger { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
+struct LargerFloat { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Plus { __device__ float operator()(float a, float b) const { return a + b; } };
+
 // An alternative: its value as an ordered word above its class, so that the largest word is
 // the most probable class and the lowest of equal ones. 0: none.
 typedef unsigned long long Alt;
@@ -32,6 +65,21 @@ __device__ __forceinline__ Alt alt_of(float x, uint32_t cls) {
 // e^z, z <= 0: v_exp_f32 gives 2^y to one unit in the last place, and 0 below 2^-126.
 __device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
 
+// The lane's number, anew: what follows from it is not kept in registers from row to row.
+__device__ __forceinline__ uint32_t lane_now() {
+    uint32_t l = __lane_id();
+    asm volatile("" : "+v"(l));
+    return l;
+}
+
+// log s, 1 <= s (or 0, or NaN): v_log_f32 gives log2 s, which two parts of log 2 take to the
+// last place.
+__device__ __forceinline__ float log_of(float s) {
+    const float l = __builtin_amdgcn_logf(s), hi = 0.693147182464599609375f, lo = -1.904654299957767e-9f;
+    const float r = l * hi;
+    return r + fmaf(l, lo, fmaf(l, hi, -r));
+}
+
 struct Sums {
     float m, s, t;
     __device__ void init() { m = kLowest; s = 0.0f; t = 0.0f; }
@@ -46,6 +94,12 @@ struct Sums {
         s += e;
         t += fmaxf(z, -200.0f) * e;     // -inf: 0 * -200; NaN goes on through e
     }
+    // the sums of the G lanes of a group, in every lane of it
+    template <int G> __device__ void join_group() {
+        raise(group_all<G>(m, LargerFloat()));
+        s = group_all<G>(s, Plus());
+        t = group_all<G>(t, Plus());
+    }
     __device__ void join(float m2, float s2, float t2) {
         Sums o{m2, s2, t2};
         const float top = fmaxf(m, m2);
@@ -53,33 +107,6 @@ struct Sums {
         o.raise(top);
         s += o.s;
         t += o.t;
-    }
-};
-
-// 64 alternatives in falling order, the i-th in lane i (0: an empty place).
-struct TopList {
-    Alt a;
-    __device__ Alt at(uint32_t lane) const {
-        return (Alt)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(a >> 32), lane) << 32 |
-               (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)a, lane);
-    }
-    // c (the same in every lane) goes behind the larger ones; the last place falls out
-    __device__ void insert(Alt c) {
-        const uint32_t lane = __lane_id();
-        const uint32_t pos = __popcll(__ballot(a > c));
-        const Alt up = __shfl_up(a, 1);
-        a = lane < pos ? a : lane == pos ? c : up;
-    }
-    // the 64 largest of both lists
-    __device__ void merge(Alt other) {
-        const uint32_t lane = __lane_id();
-        const Alt rev = __shfl(other, 63 - lane);
-        a = a > rev ? a : rev;                       // a bitonic sequence with the 64 largest
-#pragma unroll
-        for (int o = 32; o; o >>= 1) {
-            const Alt b = __shfl_xor(a, o);
-            a = (lane & o) ? (a < b ? a : b) : (a > b ? a : b);
-        }
     }
 };
 
@@ -91,8 +118,8 @@ struct RowEnd {
         m = q.m;
         bad = q.s != q.s;
         empty = q.s == 0.0f;
-        ls = logf(q.s);
-        const float e = ls - q.t / q.s;
+        ls = log_of(q.s);
+        const float e = ls - q.t * __builtin_amdgcn_rcpf(q.s);
         h = bad ? NAN : empty || e < 0.0f ? 0.0f : e;
     }
     // log p of the class whose logit is x
@@ -103,25 +130,15 @@ struct RowEnd {
     }
 };
 
-// The given class' log probability and the entropy, by one lane.
-template <int DT>
-__device__ __forceinline__ void put_row(const LogprobArgs &a, uint64_t r, const RowEnd &end) {
-    using T = typename Elem<DT>::T;
-    if (a.target) {
-        const int32_t t = a.target[r];
-        float lp = t == -1 ? 0.0f : NAN;
-        if (t >= 0 && (uint32_t)t < a.v) lp = end.log_p((float)static_cast<const T *>(a.x)[r * a.ld + (uint32_t)t]);
-        a.logprob[r] = lp;
-    }
+// The row's outputs, by a whole wave (all lanes hold the same sums); xt: the given class' logit.
+__device__ __forceinline__ void put_row(const LogprobArgs &a, uint64_t r, const RowEnd &end, int32_t target, float xt) {
+    if (a.target) a.logprob[r] = target == -1 ? 0.0f : (uint32_t)target < a.v ? end.log_p(xt) : NAN;
     if (a.entropy) a.entropy[r] = end.h;
 }
-
-// The row's outputs, by a whole wave (all lanes hold the same sums).
-template <int DT>
-__device__ void finish_row(const LogprobArgs &a, uint64_t r, const Sums &q, Alt alt) {
-    const uint32_t lane = __lane_id();
+__device__ void finish_row(const LogprobArgs &a, uint64_t r, const Sums &q, Alt alt, int32_t target, float xt) {
+    const uint32_t lane = lane_now();
     const RowEnd end(q);
-    if (lane == 0) put_row<DT>(a, r, end);
+    if (lane == 0) put_row(a, r, end, target, xt);
     if (lane < a.top) {
         a.top_id[r * a.top + lane] = end.id(alt);
         a.top_lp[r * a.top + lane] = end.id_log_p(alt);
@@ -133,144 +150,336 @@ __device__ void finish_row(const LogprobArgs &a, uint64_t r, const Sums &q, Alt 
 // Up to 64 N classes: a lane holds N neighbouring logits of its row, G lanes (a power of two)
 // a row, so the row is read once and its maximum is known before the sums. An alternative is
 // the group's largest word; its lane clears it and the next round finds the next. The lanes
-// keep the results of G rounds and store them side by side.
-template <int DT, int N, bool TOP>
-__global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t G) {
+// keep the results of G rounds and store them side by side. WHOLE: the classes are a multiple
+// of N, so a lane has all of its logits or none; the next rows are then under way while a
+// block works on the ones before.
+template <int DT, int N, int G, bool WHOLE>
+__global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a) {
     using T = typename Elem<DT>::T;
-    const uint32_t g = threadIdx.x & (G - 1), per = 256 / G, c0 = g * N;
-    for (uint64_t r0 = (uint64_t)blockIdx.x * per; r0 < a.rows; r0 += (uint64_t)gridDim.x * per) {
-        const uint64_t r = r0 + threadIdx.x / G;
+    constexpr uint32_t PER = 256 / G;
+    const uint32_t g = threadIdx.x % G, c0 = g * N;
+    const uint64_t step = (uint64_t)gridDim.x * PER;
+    uint64_t r = (uint64_t)blockIdx.x * PER + threadIdx.x / G;
+    const bool in_row = c0 < a.v;
+    T next[N];
+    int32_t next_target = -1;
+    auto fetch = [&](uint64_t row) {
+        if (a.target) next_target = a.target[row < a.rows ? row : a.rows - 1];
+        const T *p = static_cast<const T *>(a.x) + (row < a.rows ? row : a.rows - 1) * a.ld + (in_row ? c0 : 0);
+        if constexpr (WHOLE) {
+            __builtin_memcpy(next, p, sizeof(next));
+        } else {
+            const int64_t ok = (int64_t)a.v - c0;
+            if (ok >= N) __builtin_memcpy(next, p, sizeof(next));
+            else
+#pragma unroll
+                for (int i = 0; i < N; ++i) next[i] = p[i < ok ? i : 0];
+        }
+    };
+    fetch(r);
+    // (all lanes of a block go round together: its first row decides)
+    for (uint64_t b0 = (uint64_t)blockIdx.x * PER; b0 < a.rows; b0 += step, r += step) {
         const bool live = r < a.rows;
         float x[N];
-        load_row<T, N>(static_cast<const T *>(a.x) + (live ? r : 0) * a.ld + c0, live ? (int64_t)a.v - c0 : 0,
-                       -INFINITY, x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = (WHOLE ? in_row : c0 + i < a.v) ? (float)next[i] : -INFINITY;
+        const int32_t target = next_target;
+        fetch(r + step);
         Sums q;
         q.init();
 #pragma unroll
         for (int i = 0; i < N; ++i) q.m = fmaxf(q.m, x[i]);
-        for (uint32_t o = 1; o < G; o <<= 1) q.m = fmaxf(q.m, __shfl_xor(q.m, o));
+        q.m = group_all<G>(q.m, LargerFloat());
 #pragma unroll
         for (int i = 0; i < N; ++i) q.add(x[i]);
-        for (uint32_t o = 1; o < G; o <<= 1) {
-            q.s += __shfl_xor(q.s, o);
-            q.t += __shfl_xor(q.t, o);
-        }
+        q.s = group_all<G>(q.s, Plus());
+        q.t = group_all<G>(q.t, Plus());
         const RowEnd end(q);
-        if (live && g == 0) put_row<DT>(a, r, end);
-        if (!TOP) continue;
+        float xt = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; ++i) xt = target == (int32_t)(c0 + i) ? x[i] : xt;
+        xt = group_all<G>(xt, LargerFloat());
+        if (live && g == 0) put_row(a, r, end, target, xt);
+        if (a.top == 0) continue;
         uint32_t w[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = x[i] > -INFINITY ? ord_of(x[i]) : 0u;
         Alt mine = 0;
-        for (uint32_t k = 0; k < a.top; ++k) {
-            uint32_t b = 0, at = 0;
+        uint64_t to = r * a.top + g;
+        for (uint32_t k = 0;; ++k) {
+            uint32_t b = w[0], c = c0;
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (w[i] > b) { b = w[i]; at = i; }
-            Alt best = b ? (Alt)b << 32 | (uint32_t)~(c0 + at) : 0;
-            const Alt own = best;
-            for (uint32_t o = 1; o < G; o <<= 1) {
-                const Alt other = __shfl_xor(best, o);
-                best = other > best ? other : best;
-            }
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (own == best && at == (uint32_t)i) w[i] = 0;
-            const uint32_t place = k & (G - 1);
+            for (int i = 1; i < N; ++i)
+                if (w[i] > b) { b = w[i]; c = c0 + i; }
+            const Alt own = b ? (Alt)b << 32 | (uint32_t)~c : 0;
+            const Alt best = group_all<G>(own, Larger());
+            const uint32_t place = k % G;
             if (place == g) mine = best;
-            if ((place == G - 1 || k == a.top - 1) && g <= place && live) {
-                const uint64_t to = r * a.top + (k - place) + g;
-                a.top_id[to] = end.id(mine);
-                a.top_lp[to] = end.id_log_p(mine);
+            const bool last = k + 1 == a.top;
+            if (last || place == G - 1) {
+                if (g <= place && live) {
+                    a.top_id[to] = end.id(mine);
+                    a.top_lp[to] = end.id_log_p(mine);
+                }
+                if (last) break;
+                to += G;
             }
+            const uint32_t gone = (uint32_t)~(uint32_t)best;   // (in its own lane one of c0 .. c0 + N - 1)
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = gone == c0 + i ? 0 : w[i];
         }
     }
 }
 
-// ---------------------------------------------------------------- long rows: a block a row
+template <int DT, int N, int G> static bool logprobs_short(const LogprobArgs &a, hipStream_t st) {
+    const uint64_t blocks = (a.rows + 256 / G - 1) / (256 / G);
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(blocks, 256 * 8);   // (the blocks that fit at once)
+    if (a.v % N == 0) k_logprobs_short<DT, N, G, true><<<grid, 256, 0, st>>>(a);
+    else k_logprobs_short<DT, N, G, false><<<grid, 256, 0, st>>>(a);
+    return true;
+}
+// 16 bytes a lane as far as 64 lanes reach; then 16 logits a lane
+constexpr uint32_t kShort = 64 * 16;
+template <int DT> static bool logprobs_short(const LogprobArgs &a, hipStream_t st) {
+    constexpr int N = DT == FSX_DTYPE_F32 ? 4 : 8;
+    if (a.v > kShort) return false;
+    if (a.v <= 1 * N) return logprobs_short<DT, N, 1>(a, st);
+    if (a.v <= 2 * N) return logprobs_short<DT, N, 2>(a, st);
+    if (a.v <= 4 * N) return logprobs_short<DT, N, 4>(a, st);
+    if (a.v <= 8 * N) return logprobs_short<DT, N, 8>(a, st);
+    if (a.v <= 16 * N) return logprobs_short<DT, N, 16>(a, st);
+    if (a.v <= 32 * N) return logprobs_short<DT, N, 32>(a, st);
+    if (a.v <= 64 * N) return logprobs_short<DT, N, 64>(a, st);
+    if constexpr (DT == FSX_DTYPE_F32) if (a.v <= 32 * 16) return logprobs_short<DT, 16, 32>(a, st);
+    return logprobs_short<DT, 16, 64>(a, st);
+}
 
-constexpr int kLW = 4;        // waves a block
-constexpr int kLV = 8;        // neighbouring logits a lane reads
-constexpr int kLH = 4;        // such reads in flight
-constexpr uint32_t kPiece = 64 * kLV * kLH;
+// ---------------------------------------------------------------- long rows: blocks of W waves
+
+constexpr int kLV = 8;             // neighbouring logits a lane reads
 constexpr uint32_t kMaxParts = 64;
 
-// The wave's share of a row: pieces of kPiece logits, `stride` pieces apart, in rising order
-// of the classes: a later logit equal to the last alternative never replaces it.
-template <int DT, bool TOP>
-__device__ void wave_pass(const typename Elem<DT>::T *x, uint32_t v, uint32_t first, uint32_t stride, uint32_t top,
-                          Sums &q, TopList &list) {
-    const uint32_t lane = __lane_id();
-    float tau = -INFINITY;              // the last alternative kept so far; masked logits never pass
-    for (uint64_t p = (uint64_t)first * kPiece; p < v; p += (uint64_t)stride * kPiece) {
-        const uint32_t c0 = (uint32_t)p + lane * kLV;
-        float e[kLH][kLV];
+// The wave's number in its block, as the scalar that it is.
+__device__ __forceinline__ uint32_t wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// The upper 12 bits of the n-th largest of the waves' words, by each wave from ballots: when
+// they are logits of different places, no logit below it is among the n largest.
+template <int WORDS> __device__ uint32_t nth_largest(const uint32_t (&w)[WORDS], uint32_t n) {
+    uint32_t f = 0;
+#pragma unroll 1
+    for (uint32_t bit = 0x80000000u; bit >= 0x100000u; bit >>= 1) {
+        uint32_t count = 0;
 #pragma unroll
-        for (int h = 0; h < kLH; ++h) {
-            const uint32_t c = c0 + h * 64 * kLV;
-            load_row<typename Elem<DT>::T, kLV>(x + c, (int64_t)v - c, -INFINITY, e[h]);
-        }
-        float top_e = e[0][0];
-#pragma unroll
-        for (int h = 0; h < kLH; ++h)
-#pragma unroll
-            for (int i = 0; i < kLV; ++i) top_e = fmaxf(top_e, e[h][i]);
-        if (top_e > q.m) q.raise(top_e);
-#pragma unroll
-        for (int h = 0; h < kLH; ++h)
-#pragma unroll
-            for (int i = 0; i < kLV; ++i) q.add(e[h][i]);
-        const uint64_t better = TOP ? __ballot(top_e > tau) : 0;
-        if (better) {
-            // with `top` lanes better than tau, the top-th largest of the lanes' maxima is a
-            // lower bound of the last alternative after this piece: its upper 16 bits, one by one
-            uint32_t floor_w = 0;
-            if ((uint32_t)__popcll(better) >= top) {
-                const uint32_t w = top_e > tau ? ord_of(top_e) : 0;
-                for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
-                    if ((uint32_t)__popcll(__ballot(w >= (floor_w | bit))) >= top) floor_w |= bit;
-            }
-#pragma unroll
-            for (int h = 0; h < kLH; ++h)
-#pragma unroll
-                for (int i = 0; i < kLV; ++i) {
-                    Alt mine = e[h][i] > tau && ord_of(e[h][i]) >= floor_w ? alt_of(e[h][i], c0 + h * 64 * kLV + i) : 0;
-                    if (!__ballot(mine != 0)) continue;
-                    for (;;) {
-                        const uint64_t want = __ballot(mine > list.at(top - 1));
-                        if (!want) break;
-                        const uint32_t src = (uint32_t)__builtin_ctzll(want);
-                        list.insert(TopList{mine}.at(src));
-                        if (lane == src) mine = 0;
-                    }
-                }
-            const Alt last = list.at(top - 1);
-            if (last) tau = value_of((uint32_t)(last >> 32));
-        }
+        for (int i = 0; i < WORDS; ++i) count += (uint32_t)__popcll(__ballot(w[i] >= (f | bit)));
+        if (count >= n) f |= bit;
     }
-    // the wave's sums, in every lane
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const float m2 = __shfl_xor(q.m, o), s2 = __shfl_xor(q.s, o), t2 = __shfl_xor(q.t, o);
-        q.join(m2, s2, t2);
-    }
+    return f;
 }
 
-// The waves' results into the first wave's (the others keep theirs).
-template <bool TOP>
-__device__ void block_join(Sums &q, TopList &list) {
-    __shared__ float s_q[kLW][3];
-    __shared__ Alt s_list[kLW][64];
-    const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6;
-    __syncthreads();
-    if (lane == 0) { s_q[wave][0] = q.m; s_q[wave][1] = q.s; s_q[wave][2] = q.t; }
-    if (TOP) s_list[wave][lane] = list.a;
-    __syncthreads();
-    if (wave == 0)
-        for (int w = 1; w < kLW; ++w) {
-            q.join(s_q[w][0], s_q[w][1], s_q[w][2]);
-            if (TOP) list.merge(s_list[w][lane]);
+// Candidates for a row's alternatives: each wave collects its own, unordered; an order comes
+// from counting for each how many are larger (their words all differ), so no list is kept
+// sorted and no lane waits for another.
+constexpr uint32_t kPool = 128;   // a wave's candidates: 64 alternatives and one of every lane
+constexpr uint32_t kFewTop = 32;  // up to here a bound from 64 words does; beyond, from 256
+template <int W> struct Shared {
+    Alt pool[W][kPool];
+    Alt all[W * kPool];
+    Alt best[64];
+    uint32_t word[64 * W];
+    float sums[W][3];
+    uint32_t total;
+};
+struct Pool {
+    Alt *at;
+    uint32_t n;   // (the same in the wave)
+    __device__ void put(uint64_t m, bool want, Alt a) {   // m: the lanes that want
+        if (want) at[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = a;
+        n += (uint32_t)__popcll(m);
+    }
+    // only the `top` largest stay, in falling order; the last one's word (there are more than `top`)
+    __device__ uint32_t keep_best(uint32_t top) {
+        const uint32_t lane = __lane_id();
+        const Alt a = lane < n ? at[lane] : 0, b = lane + 64 < n ? at[lane + 64] : 0;
+        uint32_t ra = 0, rb = 0;
+#pragma unroll 1
+        for (uint32_t i = 0; i < n; ++i) {
+            const Alt o = at[i];
+            ra += o > a;
+            rb += o > b;
         }
+        if (a && ra < top) at[ra] = a;
+        if (b && rb < top) at[rb] = b;
+        n = top;
+        return __builtin_amdgcn_readfirstlane((uint32_t)(at[top - 1] >> 32));
+    }
+};
+
+// A lower bound of the n-th largest of what the waves' lanes put into sh.word, from 64 words
+// (each the largest of a lane of all waves) or, for many alternatives, 256.
+template <int W> __device__ __forceinline__ uint32_t bound(const Shared<W> &sh, uint32_t n) {
+    const uint32_t lane = lane_now();
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = sh.word[64 * i + lane];
+#pragma unroll
+        for (int j = i + 4; j < W; j += 4) w[i] = max(w[i], sh.word[64 * j + lane]);
+    }
+    if (n > kFewTop) return nth_largest(w, n);
+    const uint32_t one[1] = {max(max(w[0], w[1]), max(w[2], w[3]))};
+    return nth_largest(one, n);
+}
+
+// The waves' sums and pools: the block's sums in every lane, its `top` largest candidates in
+// falling order, the i-th in lane i of the first wave (0: none). sh.total was 0 before a barrier.
+template <int W, bool TOP>
+__device__ __forceinline__ Alt block_join(Shared<W> &sh, Sums &q, const Pool &pool, uint32_t top) {
+    const uint32_t lane = lane_now(), wave = wave_id();
+    if (lane == 0) {
+        sh.sums[wave][0] = q.m;
+        sh.sums[wave][1] = q.s;
+        sh.sums[wave][2] = q.t;
+    }
+    if (TOP) {
+        if (wave == 0) sh.best[lane] = 0;
+        uint32_t base = 0;
+        if (lane == 0 && pool.n) base = atomicAdd(&sh.total, pool.n);   // (any order: it ends in one by value)
+        base = __builtin_amdgcn_readfirstlane(base);
+        if (lane < pool.n) sh.all[base + lane] = pool.at[lane];
+        if (lane + 64 < pool.n) sh.all[base + lane + 64] = pool.at[lane + 64];
+    }
+    __syncthreads();
+    q.m = sh.sums[lane & (W - 1)][0];
+    q.s = sh.sums[lane & (W - 1)][1];
+    q.t = sh.sums[lane & (W - 1)][2];
+    q.template join_group<W>();
+    if (!TOP) {
+        __syncthreads();
+        return 0;
+    }
+    const uint32_t n = __builtin_amdgcn_readfirstlane(sh.total);
+#pragma unroll 1
+    for (uint32_t first = wave * 64; first < n; first += W * 64) {
+        const Alt a = first + lane < n ? sh.all[first + lane] : 0;
+        uint32_t rank = 0, i = 0;
+#pragma unroll 1
+        for (; i + 8 <= n; i += 8) {
+            Alt o[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = sh.all[i + j];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rank += o[j] > a;
+        }
+#pragma unroll 1
+        for (; i < n; ++i) rank += sh.all[i] > a;
+        if (a && rank < top) sh.best[rank] = a;
+    }
+    __syncthreads();
+    return sh.best[lane];
+}
+
+// A block's share of a row: its waves' pieces of 64 kLV H logits, in rising order of the classes,
+// so that a later logit equal to a wave's last alternative never replaces it. A logit is a
+// candidate if its ordered word is `low` at least.
+//
+// The code is kept small (one copy of each part, loops that are not unrolled): the time of a
+// short call is else that of fetching its instructions.
+template <int DT, int W, int H, bool TOP>
+__device__ __forceinline__ void block_pass(Shared<W> &sh, const typename Elem<DT>::T *x, uint32_t v, uint32_t part,
+                                           uint32_t parts, uint32_t top, Sums &q, Pool &pool) {
+    using T = typename Elem<DT>::T;
+    constexpr uint32_t kPiece = 64 * kLV * H;
+    const uint32_t lane = lane_now(), wave = wave_id();
+    q.init();
+    pool.at = sh.pool[wave];
+    pool.n = 0;
+    uint32_t low = ord_of(kLowest);   // masked logits never pass
+    uint32_t round = 0, refresh = 0;
+#pragma unroll 1
+    for (uint32_t block_at = part * W * kPiece; block_at < v; block_at += parts * W * kPiece, ++round) {   // (< 2^32)
+        const uint32_t at = block_at + wave * kPiece;
+        const bool some = at < v;
+        // the lane's reads; one that would pass the row's end (v > kLV) begins before its place and
+        // what belongs to others does not count
+        const uint32_t c0 = at + lane * kLV, end = v - kLV;
+        float e[H][kLV];
+        float top_e = -INFINITY;
+        if (some) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const uint32_t c = c0 + h * 64 * kLV;
+                T raw[kLV];
+                __builtin_memcpy(raw, x + (c < end ? c : end), sizeof(raw));
+#pragma unroll
+                for (int i = 0; i < kLV; ++i) e[h][i] = (float)raw[i];
+            }
+            if (at + kPiece > v) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    const uint32_t c = c0 + h * 64 * kLV;
+#pragma unroll
+                    for (int i = 0; i < kLV; ++i) e[h][i] = c > end && end + i < c ? -INFINITY : e[h][i];
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < kLV; ++i) top_e = fmaxf(top_e, e[h][i]);
+            if (top_e > q.m) q.raise(top_e);
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < kLV; ++i) q.add(e[h][i]);
+            asm volatile("" : "+v"(q.s), "+v"(q.t));   // (the sums are done before the candidates)
+        }
+        if (!TOP) continue;
+        // a lower bound of the block's last alternative, from its lanes' largest logits so far, in
+        // rounds 0, 1, 4, 16, 64 ..
+        if (round == refresh) {
+            if (round) __syncthreads();   // (the time before still reads the words)
+            else if (threadIdx.x == 0) sh.total = 0;
+            refresh = round ? 4 * round : 1;
+            sh.word[threadIdx.x] = ord_of(q.m);
+            __syncthreads();
+            low = max(low, bound(sh, top));
+        }
+        if (!some || !__ballot(top_e >= value_of(low))) continue;
+        const float lim = value_of(low);
+        uint32_t done = H * kLV;   // the first logit of a lane that found no room
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            float here = e[h][0];
+#pragma unroll
+            for (int i = 1; i < kLV; ++i) here = fmaxf(here, e[h][i]);
+            if (!__ballot(here >= lim)) continue;
+            const uint32_t c = c0 + h * 64 * kLV, from = c < end ? c : end;
+#pragma unroll
+            for (int i = 0; i < kLV; ++i) {
+                const uint64_t m = __ballot(e[h][i] >= lim);
+                if (!m || done < H * kLV) continue;
+                if (pool.n + (uint32_t)__popcll(m) > kPool) done = h * kLV + i;
+                else pool.put(m, e[h][i] >= lim, alt_of(e[h][i], from + i));
+            }
+        }
+        if (done == H * kLV) continue;
+        // no room: one logit of each lane at a time, read again, room made before it
+#pragma unroll 1
+        for (uint32_t i = done; i < H * kLV; ++i) {
+            const uint32_t c = c0 + i / kLV * 64 * kLV, cls = (c < end ? c : end) + i % kLV;
+            const float y = cls >= c ? (float)x[cls] : -INFINITY;
+            if (pool.n + 64 > kPool) low = max(low, pool.keep_best(top));
+            const bool want = y >= value_of(low);
+            pool.put(__ballot(want), want, alt_of(y, cls));
+        }
+        if (pool.n > top) low = max(low, pool.keep_best(top) + 1);   // (later an equal logit comes too late)
+    }
+    q.template join_group<64>();
+}
+
+// The given class and its logit, by the lanes that ask for them.
+template <int DT> __device__ __forceinline__ void given(const LogprobArgs &a, uint64_t r, int32_t &t, float &x) {
+    t = a.target ? a.target[r] : -1;
+    x = (uint32_t)t < a.v ? (float)static_cast<const typename Elem<DT>::T *>(a.x)[r * a.ld + (uint32_t)t] : 0.0f;
 }
 
 // A part's results in the workspace: its sums, then its alternatives.
@@ -285,81 +494,99 @@ struct Part {
     }
 };
 
-// A row is cut into `parts` (interleaved piece by piece), a block each; with one part the
+// A row is cut into `parts` (interleaved round by round), a block each; with one part the
 // block finishes the row.
-template <int DT, bool TOP>
-__global__ __launch_bounds__(64 * kLW) void k_logprobs_long(LogprobArgs a, uint32_t parts) {
+template <int DT, int W, int H, bool TOP>
+__global__ __launch_bounds__(64 * W, 8) void k_logprobs_long(LogprobArgs a, uint32_t parts) {
     using T = typename Elem<DT>::T;
-    const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6;
-    for (uint64_t i = blockIdx.x; i < a.rows * parts; i += gridDim.x) {
-        const uint64_t r = i / parts;
-        const uint32_t part = (uint32_t)(i - r * parts);
+    __shared__ Shared<W> sh;
+    const uint32_t part = blockIdx.x;
+#pragma unroll 1
+    for (uint64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
         Sums q;
-        TopList list{0};
-        q.init();
-        wave_pass<DT, TOP>(static_cast<const T *>(a.x) + r * a.ld, a.v, part * kLW + wave, parts * kLW, a.top, q,
-                           list);
-        block_join<TOP>(q, list);
-        if (wave) continue;
+        Pool pool;
+        block_pass<DT, W, H, TOP>(sh, static_cast<const T *>(a.x) + r * a.ld, a.v, part, parts, a.top, q, pool);
+        const Alt alt = block_join<W, TOP>(sh, q, pool, a.top);
+        if (wave_id()) continue;
+        const uint32_t lane = lane_now();
         if (parts == 1) {
-            finish_row<DT>(a, r, q, list.a);
+            int32_t t = -1;
+            float xt = 0.0f;
+            if (lane == 0) given<DT>(a, r, t, xt);
+            finish_row(a, r, q, alt, t, xt);
         } else {
-            const Part to(a, i);
+            const Part to(a, r * parts + part);
             if (lane == 0) { to.sums[0] = q.m; to.sums[1] = q.s; to.sums[2] = q.t; }
-            if (TOP && lane < a.top) to.alts[lane] = list.a;
+            if (TOP && lane < a.top) to.alts[lane] = alt;
         }
     }
 }
 
+// The parts of a row: a lane of the first wave takes a part's sums; the waves take the parts'
+// alternatives in turn, above a lower bound from the first few of every part.
 template <int DT, bool TOP>
-__global__ __launch_bounds__(64 * kLW) void k_logprobs_join(LogprobArgs a, uint32_t parts) {
-    const uint32_t lane = __lane_id(), wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(256) void k_logprobs_join(LogprobArgs a, uint32_t parts) {
+    constexpr int W = 4;
+    __shared__ Shared<W> sh;
+    const uint32_t lane = __lane_id(), wave = wave_id();
     for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         Sums q;
-        TopList list{0};
+        Pool pool{sh.pool[wave], 0};
         q.init();
-        for (uint32_t p = wave; p < parts; p += kLW) {
-            const Part from(a, r * parts + p);
-            q.join(from.sums[0], from.sums[1], from.sums[2]);
-            if (TOP) list.merge(lane < a.top ? from.alts[lane] : 0);
+        int32_t t = -1;
+        float xt = 0.0f;
+        if (threadIdx.x == 0) given<DT>(a, r, t, xt);
+        if (TOP) {
+            const uint32_t per = (a.top > kFewTop ? 256 : 64) / parts, nth = threadIdx.x / parts;
+            const Alt sample = nth < a.top && nth < per ? Part(a, r * parts + threadIdx.x % parts).alts[nth] : 0;
+            __syncthreads();   // (the row before still reads the words)
+            if (threadIdx.x == 0) sh.total = 0;
+            sh.word[threadIdx.x] = (uint32_t)(sample >> 32);
         }
-        block_join<TOP>(q, list);
-        if (wave == 0) finish_row<DT>(a, r, q, list.a);
+        if (wave == 0 && lane < parts) {
+            const Part from(a, r * parts + lane);
+            q.join(from.sums[0], from.sums[1], from.sums[2]);
+        }
+        q.template join_group<64>();
+        if (TOP) {
+            __syncthreads();
+            const uint32_t low = bound(sh, a.top);
+#pragma unroll 1
+            for (uint32_t p = wave; p < parts; p += 4 * W) {
+                Alt mine[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    mine[j] = p + j * W < parts && lane < a.top ? Part(a, r * parts + p + j * W).alts[lane] : 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (pool.n + 64 > kPool) pool.keep_best(a.top);
+                    const bool want = mine[j] != 0 && (uint32_t)(mine[j] >> 32) >= low;
+                    pool.put(__ballot(want), want, mine[j]);
+                }
+            }
+        }
+        const Alt alt = block_join<W, TOP>(sh, q, pool, a.top);
+        if (wave == 0) finish_row(a, r, q, alt, t, xt);
     }
 }
 
-// Lanes a row and logits a lane of the short form; N 0: the long form.
-struct ShortPlan {
-    uint32_t n, g;
-};
-template <int DT> static ShortPlan short_plan(uint32_t v) {
-    constexpr uint32_t wide = DT == FSX_DTYPE_F32 ? 4 : 8;   // 16 bytes a lane
-    ShortPlan p{v <= 64 * wide ? wide : v <= 64 * 16 ? 16u : 0u, 1};
-    while (p.n && p.g * p.n < v) p.g *= 2;
-    return p;
-}
-
-// Parts of a long row: enough blocks for every CU to hold four, a piece for every wave at least.
+// Many rows: a block of four waves each. Fewer: of sixteen, each with less to do, and with
+// fewer rows than half the CUs a row in parts, a round for every block at least.
+static constexpr uint64_t kManyRows = 1024;
+static constexpr int kFewW = 16, kFewH = 1;
 static uint32_t long_parts(uint64_t rows, uint32_t v) {
-    if (v <= 64 * 16) return 1;
-    const uint64_t want = (1024 + rows - 1) / rows, most = (v + kPiece * kLW - 1) / (kPiece * kLW);
-    return (uint32_t)std::min<uint64_t>({want, most, kMaxParts});
+    if (v <= kShort || rows >= kManyRows) return 1;
+    const uint64_t want = (256 + rows / 2) / rows, most = (v + 64 * kLV * kFewH * kFewW - 1) / (64 * kLV * kFewH * kFewW);
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({want, most, kMaxParts}));
 }
 
 template <int DT, bool TOP>
 static void logprobs(const LogprobArgs &a, hipStream_t st) {
-    const ShortPlan p = short_plan<DT>(a.v);
-    if (p.n) {
-        const uint64_t blocks = (a.rows + 256 / p.g - 1) / (256 / p.g);
-        const uint32_t grid = (uint32_t)std::min<uint64_t>(blocks, 1u << 16);
-        if (p.n == 16) k_logprobs_short<DT, 16, TOP><<<grid, 256, 0, st>>>(a, p.g);
-        else k_logprobs_short<DT, DT == FSX_DTYPE_F32 ? 4 : 8, TOP><<<grid, 256, 0, st>>>(a, p.g);
-        return;
-    }
     const uint32_t parts = long_parts(a.rows, a.v);
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(a.rows * parts, 1u << 20);
-    k_logprobs_long<DT, TOP><<<grid, 64 * kLW, 0, st>>>(a, parts);
-    if (parts > 1) k_logprobs_join<DT, TOP><<<(uint32_t)std::min<uint64_t>(a.rows, 1u << 16), 64 * kLW, 0, st>>>(a, parts);
+    const dim3 grid(parts, (uint32_t)std::min<uint64_t>(a.rows, 65535));
+    if (a.rows >= kManyRows) k_logprobs_long<DT, 4, 4, TOP><<<grid, 64 * 4, 0, st>>>(a, 1);
+    else k_logprobs_long<DT, kFewW, kFewH, TOP><<<grid, 64 * kFewW, 0, st>>>(a, parts);
+    if (parts > 1) k_logprobs_join<DT, TOP><<<(uint32_t)std::min<uint64_t>(a.rows, 1u << 16), 256, 0, st>>>(a, parts);
 }
 
 uint64_t logprobs_work(uint64_t rows, uint32_t v, uint32_t top) {
@@ -369,6 +596,7 @@ uint64_t logprobs_work(uint64_t rows, uint32_t v, uint32_t top) {
 
 template <int DT>
 static void logprobs(const LogprobArgs &a, hipStream_t st) {
+    if (logprobs_short<DT>(a, st)) return;
     if (a.top) logprobs<DT, true>(a, st);
     else logprobs<DT, false>(a, st);
 }
