@@ -395,24 +395,33 @@ __device__ __forceinline__ void block_pass(Shared<W> &sh, const typename Elem<DT
     pool.n = 0;
     uint32_t low = ord_of(kLowest);   // masked logits never pass
     uint32_t round = 0, refresh = 0;
+    // the lane's reads; one that would pass the row's end (v > kLV) begins before its place and
+    // what belongs to others does not count
+    const uint32_t end = v - kLV, step = parts * W * kPiece;
+    T raw[H][kLV];
+    auto read = [&](uint32_t c0) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const uint32_t c = c0 + h * 64 * kLV;
+            __builtin_memcpy(raw[h], x + (c < end ? c : end), sizeof(raw[h]));
+        }
+    };
+    constexpr bool AHEAD = H == 1;   // (with more reads a lane the registers go to more waves)
+    if (AHEAD) read((part * W + wave) * kPiece + lane * kLV);
 #pragma unroll 1
-    for (uint32_t block_at = part * W * kPiece; block_at < v; block_at += parts * W * kPiece, ++round) {   // (< 2^32)
+    for (uint32_t block_at = part * W * kPiece; block_at < v; block_at += step, ++round) {   // (< 2^32)
         const uint32_t at = block_at + wave * kPiece;
         const bool some = at < v;
-        // the lane's reads; one that would pass the row's end (v > kLV) begins before its place and
-        // what belongs to others does not count
-        const uint32_t c0 = at + lane * kLV, end = v - kLV;
+        const uint32_t c0 = at + lane * kLV;
         float e[H][kLV];
         float top_e = -INFINITY;
         if (some) {
+            if (!AHEAD) read(c0);
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                const uint32_t c = c0 + h * 64 * kLV;
-                T raw[kLV];
-                __builtin_memcpy(raw, x + (c < end ? c : end), sizeof(raw));
+            for (int h = 0; h < H; ++h)
 #pragma unroll
-                for (int i = 0; i < kLV; ++i) e[h][i] = (float)raw[i];
-            }
+                for (int i = 0; i < kLV; ++i) e[h][i] = (float)raw[h][i];
+            if (AHEAD) read(c0 + step);   // (behind the row: its end once more, unused)
             if (at + kPiece > v) {
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
