@@ -33,11 +33,11 @@ COMMON = [
 LIBS = {
     "libfsx_hip.so": ["fsx_device.hip", "fsx_limiters.hip", "fsx_shard.hip", "fsx_pcap.hip",
                       "fsx_flows.hip", "fsx_score.hip", "fsx_heavy.hip",
-                      "fsx_linear.hip", "fsx_logprobs.hip", "fsx_api.hip"],
+                      "fsx_quantize.hip", "fsx_narrow.hip", "fsx_linear.hip", "fsx_logprobs.hip", "fsx_api.hip"],
     "libfsx_synth.so": ["fsx_synth.hip"],
 }
 HEADERS = ["fsx_internal.h", "fsx_synth_common.h", "fsx_dev_common.h", "fsx_q8.h", "fsx_seg.h", "fsx_shard.h", "fsx_walk.h",
-           "fsx_flow_common.h", "fsx_heavy_view.h", "fsx_search.h", "fsx_plan.h", "fsx_head.h"]
+           "fsx_flow_common.h", "fsx_heavy_view.h", "fsx_search.h", "fsx_plan.h", "fsx_head.h", "fsx_q8_rows.h"]
 
 
 def _stale(out: Path, srcs: list[Path]) -> bool:
@@ -75,7 +75,7 @@ def build_lib(name: str, force: bool = False, verbose: bool = False,
     with ThreadPoolExecutor(jobs) as ex:
         list(ex.map(lambda so: _compile(so[0], so[1], list(extra or [])), zip(srcs, objs)))
     tmp = out.with_suffix(".so.tmp")
-    cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
+    cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-Wl,--no-undefined", "-o", str(tmp), *map(str, objs)]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc link failed for {name}:\n{r.stdout}\n{r.stderr}")

@@ -1751,7 +1751,8 @@ static bool layer_sizes_ok(const fsx_q8_linear *l) {
 size_t fsx_linear_q8_work(const fsx_q8_linear *layer, int x_dtype, size_t rows) {
     if (!layer_sizes_ok(layer) || rows == 0 || rows > kMaxRows || layer->out_features == 0) return 0;
     if (x_dtype != FSX_DTYPE_I8 && !float_type(x_dtype)) return 0;
-    return linear_work(rows, (uint32_t)layer->in_features, (uint32_t)layer->out_features, x_dtype);
+    return linear_work(rows, (uint32_t)layer->in_features, (uint32_t)layer->out_features, x_dtype, nullptr, 0,
+                       layer->weight, layer->ld_weight);
 }
 
 int fsx_linear_q8_device(fsx_ctx *c, const fsx_q8_linear *layer, const void *d_x, int x_dtype, size_t ldx,
@@ -1775,7 +1776,8 @@ int fsx_linear_q8_device(fsx_ctx *c, const fsx_q8_linear *layer, const void *d_x
     if (!rc && x_dtype == FSX_DTYPE_I8) rc = check_matrix(c, "x scales", d_x_scale, 4, rows, 1, 1);
     if (!rc && x_dtype != FSX_DTYPE_I8 && d_x_scale) rc = set_err(c, -EINVAL, "x scales given for float rows");
     if (!rc) rc = check_matrix(c, "y", d_y, elem_size(y_dtype), rows, n, ldy);
-    if (!rc) rc = check_work(c, d_work, work_bytes, linear_work(rows, (uint32_t)k, (uint32_t)n, x_dtype));
+    if (!rc) rc = check_work(c, d_work, work_bytes, linear_work(rows, (uint32_t)k, (uint32_t)n, x_dtype, d_x, ldx,
+                                                                layer->weight, layer->ld_weight));
     if (!rc) rc = sel(c);
     if (rc) return rc;
     LinearArgs a{};

@@ -1,4 +1,5 @@
-// fsx_head.h — heads of free size (fsx_linear.hip, fsx_logprobs.hip): element types, the host
+// fsx_head.h — heads of free size (fsx_quantize.hip, fsx_linear.hip, fsx_narrow.hip,
+// fsx_logprobs.hip): element types, the host
 // rules that the *_work functions and the launches share, and the launch functions.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -57,7 +58,9 @@ struct LogprobArgs {
 
 hipError_t launch_quantize_rows(const void *x, int dtype, uint64_t rows, uint32_t cols, uint64_t ldx, int8_t *q,
                                 uint64_t ldq, float *scale, hipStream_t st);
-uint64_t linear_work(uint64_t rows, uint32_t k, uint32_t n, int x_dtype);
+void launch_linear_narrow(const LinearArgs &a, int x_dtype, int y_dtype, hipStream_t st);   // k <= 64
+uint64_t linear_work(uint64_t rows, uint32_t k, uint32_t n, int x_dtype, const void *x, uint64_t ldx, const void *w,
+                     uint64_t ldw);
 hipError_t launch_linear(const LinearArgs &a, int x_dtype, int y_dtype, void *work, hipStream_t st);
 uint64_t logprobs_work(uint64_t rows, uint32_t v, uint32_t top);
 hipError_t launch_logprobs(const LogprobArgs &a, int dtype, hipStream_t st);
@@ -86,6 +89,35 @@ __device__ __forceinline__ void load_row(const T *p, int64_t ok, float fill, flo
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = i < ok ? (float)t[i] : fill;
     }
+}
+// The value of lane ^ O, without LDS where the hardware has a lane permutation for it.
+template <int O> __device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
+    static_assert(O == 1 || O == 2 || O == 4 || O == 8 || O == 16 || O == 32, "one bit");
+    if constexpr (O == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);          // quad_perm 1 0 3 2
+    else if constexpr (O == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);     // quad_perm 2 3 0 1
+    else if constexpr (O == 4) return __builtin_amdgcn_ds_swizzle(v, 0x101F);                // xor 4
+    else if constexpr (O == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, true);    // row_ror 8
+    else if constexpr (O == 16) return __builtin_amdgcn_ds_swizzle(v, 0x401F);               // xor 16
+    else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return __lane_id() < 32 ? r[1] : r[0];
+    }
+}
+template <int O> __device__ __forceinline__ float xor_lane(float v) {
+    return __uint_as_float(xor_lane<O>(__float_as_uint(v)));
+}
+template <int O> __device__ __forceinline__ unsigned long long xor_lane(unsigned long long v) {
+    return (unsigned long long)xor_lane<O>((uint32_t)(v >> 32)) << 32 | xor_lane<O>((uint32_t)v);
+}
+// f over the G lanes (a power of two) of a group, in every lane of it
+template <int G, typename T, typename F> __device__ __forceinline__ T group_all(T v, F f) {
+    if constexpr (G > 1) v = f(v, xor_lane<1>(v));
+    if constexpr (G > 2) v = f(v, xor_lane<2>(v));
+    if constexpr (G > 4) v = f(v, xor_lane<4>(v));
+    if constexpr (G > 8) v = f(v, xor_lane<8>(v));
+    if constexpr (G > 16) v = f(v, xor_lane<16>(v));
+    if constexpr (G > 32) v = f(v, xor_lane<32>(v));
+    return v;
 }
 #endif
 

@@ -6,127 +6,136 @@
 #include <hip/hip_runtime.h>
 #include <algorithm>
 
-#include "fsx_head.h"
+#include "fsx_q8_rows.h"
 
 namespace fsx {
 
-typedef int v4i __attribute__((ext_vector_type(4)));
-typedef int v16i __attribute__((ext_vector_type(16)));
-
-// ---------------------------------------------------------------- row quantiser
-
-constexpr float kMinScale = 1.17549435e-38f;   // 2^-126
-
-// The row's scale from its largest |x| (NaN or infinite: NaN). The quotient rounds once: a
-// 53-bit quotient of 24-bit numbers rounded to 24 bits is the 24-bit quotient.
-__device__ __forceinline__ float row_scale(float amax) {
-    if (!(amax < INFINITY)) return NAN;
-    return fmaxf(amax / 127.0f, kMinScale);
-}
-
-// rhe(x / s), exactly, of x >= 0. rint(x * (1/s)) is wrong only where x / s lies within 2^-15
-// of a half: x / s <= 127.5 and the product's relative error is below 2^-22. There the
-// remainder x - lo s decides, lo = floor(x / s): it is exact in 32 bits (lo = 0: x itself;
-// else a multiple of the last place of s, about s / 2 in size), so comparing it with s / 2
-// finds the border itself.
-__device__ __forceinline__ float code_mag(float x, float inv, float s) {
-    const float v = x * inv;
-    float r = rintf(v);
-    if (fabsf(v - r) > 0.49996f) {
-        const float lo = floorf(v), rem = fmaf(-lo, s, x), h = 0.5f * s;
-        r = rem > h || (rem == h && ((int)lo & 1)) ? lo + 1.0f : lo;
-    }
-    return r;
-}
-__device__ __forceinline__ int code_of(float x, float inv, float s) {
-    return (int)copysignf(code_mag(fabsf(x), inv, s), x);
-}
-
-// NaN if any value of the row was NaN or infinite (a NaN is lost by fmaxf: it is counted in)
-__device__ __forceinline__ float amax_of(float m, float x) {
-    const float a = fabsf(x);
-    return a > m || a != a ? a : m;      // once NaN, `a > m` is false and m stays NaN
-}
-
-constexpr int kQV = 16;   // codes a thread makes at a time: one 16-byte store
-
-// A group of TPR threads takes a row. The row is read twice; the second read comes from cache.
-template <int DT, int TPR>
-__global__ __launch_bounds__(256) void k_quantize_rows(const void *__restrict__ xp, uint64_t rows, uint32_t cols,
-                                                       uint64_t ldx, int8_t *__restrict__ q, uint64_t ldq,
-                                                       float *__restrict__ scale) {
-    using T = typename Elem<DT>::T;
-    constexpr uint32_t RPB = 256 / TPR;
-    __shared__ float s_max[4];
-    const uint32_t t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
-    for (uint64_t r0 = (uint64_t)blockIdx.x * RPB; r0 < rows; r0 += (uint64_t)gridDim.x * RPB) {
-        const uint64_t r = r0 + sub;
-        const bool live = r < rows;
-        const T *x = static_cast<const T *>(xp) + (live ? r : 0) * ldx;
-        float m = 0.0f;
-        if (live)
-            for (uint32_t c = t * kQV; c < cols; c += TPR * kQV) {
-                float v[kQV];
-                load_row<T, kQV>(x + c, (int64_t)cols - c, 0.0f, v);
-#pragma unroll
-                for (int i = 0; i < kQV; ++i) m = amax_of(m, v[i]);
-            }
-#pragma unroll
-        for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) m = amax_of(m, __shfl_xor(m, o));
-        if (TPR > 64) {
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
-            __syncthreads();
-            m = 0.0f;
-#pragma unroll
-            for (int w = 0; w < TPR / 64; ++w) m = amax_of(m, s_max[sub * (TPR / 64) + w]);
-        }
-        if (!live) continue;
-        const float s = row_scale(m);
-        const bool ok = s == s;
-        const float inv = ok ? 1.0f / s : 0.0f;
-        if (t == 0) scale[r] = s;
-        int8_t *qr = q + r * ldq;
-        for (uint32_t c = t * kQV; c < cols; c += TPR * kQV) {
-            float v[kQV];
-            int8_t o[kQV];
-            load_row<T, kQV>(x + c, (int64_t)cols - c, 0.0f, v);
-#pragma unroll
-            for (int i = 0; i < kQV; ++i) o[i] = ok ? (int8_t)code_of(v[i], inv, s) : (int8_t)0;
-            if (cols - c >= kQV) __builtin_memcpy(qr + c, o, kQV);
-            else
-#pragma unroll
-                for (int i = 0; i < kQV; ++i) if (c + i < cols) qr[c + i] = o[i];
-        }
-    }
-}
-
-template <int DT>
-static void quantize_rows(const void *x, uint64_t rows, uint32_t cols, uint64_t ldx, int8_t *q, uint64_t ldq,
-                          float *scale, hipStream_t st) {
-    const uint32_t per = (cols + kQV - 1) / kQV;   // threads that have a chunk of the row
-    auto go = [&](auto kernel, uint32_t tpr) {
-        const uint64_t blocks = (rows + 256 / tpr - 1) / (256 / tpr);
-        kernel<<<(uint32_t)std::min<uint64_t>(blocks, 1u << 16), 256, 0, st>>>(x, rows, cols, ldx, q, ldq, scale);
-    };
-    if (per <= 1) go(k_quantize_rows<DT, 1>, 1);
-    else if (per <= 4) go(k_quantize_rows<DT, 4>, 4);
-    else if (per <= 16) go(k_quantize_rows<DT, 16>, 16);
-    else if (per <= 64) go(k_quantize_rows<DT, 64>, 64);
-    else go(k_quantize_rows<DT, 256>, 256);
-}
-
-hipError_t launch_quantize_rows(const void *x, int dtype, uint64_t rows, uint32_t cols, uint64_t ldx, int8_t *q,
-                                uint64_t ldq, float *scale, hipStream_t st) {
-    (void)hipGetLastError();
-    if (rows == 0) return hipSuccess;
-    if (dtype == FSX_DTYPE_F32) quantize_rows<FSX_DTYPE_F32>(x, rows, cols, ldx, q, ldq, scale, st);
-    else if (dtype == FSX_DTYPE_F16) quantize_rows<FSX_DTYPE_F16>(x, rows, cols, ldx, q, ldq, scale, st);
-    else quantize_rows<FSX_DTYPE_BF16>(x, rows, cols, ldx, q, ldq, scale, st);
-    return hipGetLastError();
-}
+constexpr int kSums = -1;   // results that are sums still
 
 // ---------------------------------------------------------------- int8 product
+
+// ---- few rows: the weights' bytes bound it
+//
+// A block takes 16 channels and all of k, its FW waves 128 bytes of k (whole lines) each in turn,
+// straight from memory into v_mfma_i32_16x16x64_i8, the weights first: lane l gives bytes
+// 16 (l / 16) .. of row l % 16 of either operand and holds channels 4 (l / 16) .. of row l % 16
+// of the result. MT groups of 16 rows; the waves' sums meet in LDS. FLOATS: up to four rows of
+// floats, quantised by every block into LDS while its first weights are under way (x is small
+// and comes from cache): one launch instead of two.
+constexpr int kFU = 8;          // loads of weights in flight a lane
+constexpr uint32_t kFusedRows = 4, kFusedBytes = 32768;
+
+template <int XT, int MT, int FW>
+__global__ __launch_bounds__(64 * FW) void k_linear_few(LinearArgs a, int yt) {
+    constexpr bool FLOATS = XT != FSX_DTYPE_I8;
+    constexpr uint32_t THREADS = 64 * FW;
+    extern __shared__ __attribute__((aligned(16))) int8_t s_x[];   // FLOATS: the rows' codes, up64(k) + 16 apart
+    __shared__ __attribute__((aligned(16))) v4i s_acc[FW][MT][64];
+    __shared__ uint32_t s_max[kFusedRows];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15,
+                   lq = lane >> 4;
+    const uint64_t n0 = (uint64_t)blockIdx.x * 16, c = n0 + lr < a.n ? n0 + lr : a.n - 1;
+    const uint32_t chunks = (a.k + 63) / 64, pitch = chunks * 64 + 16;
+    const int8_t *pw = a.w + c * a.ldw + 16 * lq;
+    // the wave's u-th load of round t: the place in k of 64 bytes
+    auto place = [&](uint32_t t, int u) { return (2 * (wave + FW * (t * (kFU / 2) + u / 2)) + u % 2) * 64; };
+    auto load = [&](const int8_t *p, uint32_t k0) {
+        return k0 + 64 <= a.k ? load16(p + k0, 16) : load16(p + k0, (int64_t)a.k - k0 - 16 * lq);
+    };
+    v4i w[kFU];
+    auto weights = [&](uint32_t t) {
+#pragma unroll
+        for (int u = 0; u < kFU; ++u) w[u] = load(pw, place(t, u));
+    };
+    weights(0);
+    if constexpr (FLOATS) {
+        const auto *x = static_cast<const typename Elem<XT>::T *>(a.x);
+        const uint32_t per = chunks * 4, all = (uint32_t)a.rows * per;   // chunks of 16, zeros behind the end
+        if (threadIdx.x < kFusedRows) s_max[threadIdx.x] = 0;
+        __syncthreads();
+        RawChunk<XT> first;   // (kept: rows of up to 16 THREADS values are read once)
+        auto each = [&](auto f) {
+            for (uint32_t q0 = 0; q0 < all; q0 += THREADS) {
+                const uint32_t q = q0 + threadIdx.x, r = q < all ? q / per : 0, k0 = (q - r * per) * 16;
+                f(q0, q < all, r, k0, q < all && k0 < a.k);
+            }
+        };
+        each([&](uint32_t q0, bool, uint32_t r, uint32_t k0, bool some) {
+            RawChunk<XT> raw;
+            uint32_t m = 0;
+            if (some) {
+                raw.load(x + r * a.ldx + k0, (int64_t)a.k - k0);
+                m = raw.mag();
+            }
+            if (q0 == 0) first = raw;
+            const uint32_t r0 = __builtin_amdgcn_readfirstlane(r);
+            if (__ballot(some && r != r0) == 0) {
+                m = group_all<64>(m, LargerWord());
+                if (lane == 0) atomicMax(&s_max[r0], m);
+            } else if (some) {
+                atomicMax(&s_max[r], m);
+            }
+        });
+        __syncthreads();
+        each([&](uint32_t q0, bool in, uint32_t r, uint32_t k0, bool some) {
+            const float s = row_scale(mag_value<XT>(s_max[r]));
+            v4i codes = {0, 0, 0, 0};
+            if (some && s == s) {
+                RawChunk<XT> raw = first;
+                if (q0) raw.load(x + r * a.ldx + k0, (int64_t)a.k - k0);
+                codes = raw.codes(1.0f / s, s);
+            }
+            if (in) *reinterpret_cast<v4i *>(s_x + r * pitch + k0) = codes;
+        });
+        __syncthreads();
+    }
+    v4i acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = v4i{0, 0, 0, 0};
+    for (uint32_t t = 0; place(t, 0) < a.k; ++t) {
+        if (t) weights(t);
+#pragma unroll
+        for (int u = 0; u < kFU; ++u) {
+            const uint32_t k0 = place(t, u);
+            if (k0 >= a.k) break;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const uint32_t r = 16 * m + lr, rr = r < a.rows ? r : (uint32_t)a.rows - 1;
+                v4i x;
+                if (FLOATS) x = *reinterpret_cast<const v4i *>(s_x + rr * pitch + k0 + 16 * lq);
+                else x = load(static_cast<const int8_t *>(a.x) + rr * a.ldx + 16 * lq, k0);
+                acc[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u], x, acc[m], 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) s_acc[wave][m][lane] = acc[m];
+    __syncthreads();
+    if (wave >= MT) return;
+    v4i sum = s_acc[0][wave][lane];
+#pragma unroll
+    for (int i = 1; i < FW; ++i) sum += s_acc[i][wave][lane];
+    const uint64_t r = 16 * wave + lr;
+    if (r >= a.rows) return;
+    float xs;
+    if constexpr (FLOATS) xs = row_scale(mag_value<XT>(s_max[r]));
+    else xs = a.x_scale[r];
+    put_sums(a, yt, sum, xs, r, n0 + 4 * lq);
+}
+
+template <int XT, int MT> static void linear_few(const LinearArgs &a, uint32_t lds, int yt, hipStream_t st) {
+    const uint32_t blocks = (a.n + 15) / 16;
+    // us of one row, 4096 / 8192 / 16384 channels of 4096: eight waves 6.4 / 9.1 / 16.8, sixteen
+    // 5.9 / 10.9 / 20.0
+    if (blocks >= 512) k_linear_few<XT, MT, 8><<<blocks, 512, lds, st>>>(a, yt);
+    else k_linear_few<XT, MT, 16><<<blocks, 1024, lds, st>>>(a, yt);
+}
+template <int XT> static void linear_few(const LinearArgs &a, int yt, hipStream_t st) {
+    if constexpr (XT != FSX_DTYPE_I8)
+        linear_few<XT, 1>(a, (uint32_t)a.rows * ((a.k + 63) / 64 * 64 + 16), yt, st);
+    else if (a.rows <= 16) linear_few<XT, 1>(a, 0, yt, st);
+    else linear_few<XT, 2>(a, 0, yt, st);
+}
 
 // The tiles of a product over the launch's blocks. Blocks go to the 8 XCDs in turn, each with
 // an L2 of its own: an XCD takes a run of neighbouring tiles, and within it groups of kGroup
@@ -145,354 +154,113 @@ struct TileGrid {
     }
 };
 
-// 16 code bytes from p on, of which the first `ok` exist; the others are 0.
-__device__ __forceinline__ v4i load16(const int8_t *p, int64_t ok) {
-    v4i v = {0, 0, 0, 0};
-    if (ok >= 16) {
-        __builtin_memcpy(&v, p, 16);
-    } else if (ok > 0) {
-        int8_t b[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) b[i] = p[i < ok ? i : 0];   // (no conditions: all under way at once)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) b[i] = i < ok ? b[i] : (int8_t)0;
-        __builtin_memcpy(&v, b, 16);
-    }
-    return v;
-}
-
-__device__ __forceinline__ float scaled(int acc, float xs, float ws, float b) { return (float)acc * xs * ws + b; }
-__device__ __forceinline__ float relu(float y) { return y < 0.0f ? 0.0f : y; }   // NaN stays
-__device__ __forceinline__ float sigmoid(float y) {
-    const float e = expf(-fabsf(y));   // never above 1: no overflow far below 0
-    return (y >= 0.0f ? 1.0f : e) / (1.0f + e);
-}
-
-// Four neighbouring channels of one row, of which the first `ok` exist.
-template <typename T>
-__device__ __forceinline__ void store4(T *p, const float (&v)[4], int64_t ok) {
-    T t[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = (T)v[i];
-    if (ok >= 4) __builtin_memcpy(p, t, sizeof(t));
-    else
-#pragma unroll
-        for (int i = 0; i < 4; ++i) if (i < ok) p[i] = t[i];
-}
-
-template <typename T>
-__device__ __forceinline__ void store4(void *y, uint64_t at, const float (&v)[4], int64_t ok) {
-    store4(static_cast<T *>(y) + at, v, ok);
-}
-__device__ __forceinline__ void store4(void *y, int yt, uint64_t at, const float (&v)[4], int64_t ok) {
-    if (yt == FSX_DTYPE_F32) store4<float>(y, at, v, ok);
-    else if (yt == FSX_DTYPE_F16) store4<_Float16>(y, at, v, ok);
-    else store4<__bf16>(y, at, v, ok);
-}
-
-// Four neighbouring channels' scales and biases; channels behind the last: the last one's.
-struct Channels {
-    float ws[4], b[4];
-    __device__ __forceinline__ void load(const LinearArgs &a, uint64_t c) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint64_t cc = c + e < a.n ? c + e : a.n - 1;
-            ws[e] = a.w_scale[cc];
-            b[e] = a.bias ? a.bias[cc] : 0.0f;
-        }
-    }
-    __device__ __forceinline__ void finish(const LinearArgs &a, int yt, const v4i &acc, float xs, uint64_t r,
-                                           uint64_t c) const {
-        if (r >= a.rows || c >= a.n) return;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = scaled(acc[e], xs, ws[e], b[e]);
-        if (a.act == FSX_ACT_RELU) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = relu(v[e]);
-        } else if (a.act == FSX_ACT_SIGMOID) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = sigmoid(v[e]);
-        }
-        store4(a.y, yt, r * a.ldy + c, v, (int64_t)a.n - (int64_t)c);
-    }
-};
-
-// Codes of up to 16 values of a row.
-__device__ __forceinline__ v4i pack_codes(const float (&v)[kQV], float inv, float s, bool ok) {
-    v4i q;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        uint32_t u = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            u |= (uint32_t)(ok ? code_of(v[4 * w + i], inv, s) & 255 : 0) << (8 * i);
-        q[w] = (int)u;
-    }
-    return q;
-}
-
-// ---- up to 64 of k: x in registers, floats quantised there
-//
-// v_mfma_i32_16x16x64_i8, the weights first: lane l gives bytes 16 (l / 16) .. of row l % 16 of
-// either operand and holds channels 4 (l / 16) .. of row l % 16 of the result. A row of x is CH
-// chunks of 16, so a wave's lanes hold 64 / CH rows, a chunk each, in 4 / CH groups of 16 rows.
-// The weights' chunks are repeated for every group; a group is multiplied with the other
-// groups' lanes 0. x is read and y written once (the weights stay in registers), which bounds
-// it: 2^22 rows of 8 floats to 16 floats.
-template <int XT, int CH, int TN>
-__global__ __launch_bounds__(256) void k_linear_narrow(LinearArgs a, int yt) {
-    constexpr int GROUPS = 4 / CH;
-    const uint32_t lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
-    const uint32_t n0 = blockIdx.y * (16 * TN);
-    const uint32_t chunk = lq % CH, my_group = lq / CH;
-    v4i w[TN];
-    Channels ch[TN];
-#pragma unroll
-    for (int i = 0; i < TN; ++i) {
-        const uint64_t c = n0 + 16 * i + lr;
-        w[i] = load16(a.w + (c < a.n ? c : a.n - 1) * a.ldw + 16 * chunk, (int64_t)a.k - 16 * chunk);
-        ch[i].load(a, n0 + 16 * i + 4 * lq);
-    }
-    const uint64_t step = (uint64_t)gridDim.x * 4 * 16 * GROUPS;
-    for (uint64_t r0 = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 * GROUPS; r0 < a.rows; r0 += step) {
-        const uint64_t r = r0 + 16 * my_group + lr, rr = r < a.rows ? r : a.rows - 1;
-        const int64_t ok = (int64_t)a.k - 16 * chunk;
-        v4i x;
-        float xs;
-        if constexpr (XT == FSX_DTYPE_I8) {
-            x = load16(static_cast<const int8_t *>(a.x) + rr * a.ldx + 16 * chunk, ok);
-            xs = a.x_scale[rr];
-        } else {
-            using T = typename Elem<XT>::T;
-            float v[kQV];
-            load_row<T, kQV>(static_cast<const T *>(a.x) + rr * a.ldx + 16 * chunk, ok, 0.0f, v);
-            float m = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kQV; ++i) m = amax_of(m, v[i]);
-            if (CH > 1) m = amax_of(m, __shfl_xor(m, 16));
-            if (CH > 2) m = amax_of(m, __shfl_xor(m, 32));
-            xs = row_scale(m);
-            x = pack_codes(v, 1.0f / xs, xs, xs == xs);
-        }
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            v4i xg;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) xg[e] = GROUPS == 1 || my_group == (uint32_t)g ? x[e] : 0;
-            const float s = GROUPS == 1 ? xs : __shfl(xs, g * CH * 16 + lr);
-#pragma unroll
-            for (int i = 0; i < TN; ++i) {
-                const v4i acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], xg, v4i{0, 0, 0, 0}, 0, 0, 0);
-                ch[i].finish(a, yt, acc, s, r0 + 16 * g + lr, n0 + 16 * i + 4 * lq);
-            }
-        }
-    }
-}
-
-template <int XT, int CH> static void linear_narrow(const LinearArgs &a, int yt, hipStream_t st) {
-    const uint64_t waves = (a.rows + 16 * (4 / CH) - 1) / (16 * (4 / CH));
-    const uint32_t tn = a.n <= 16 ? 1 : 4, gy = (a.n + 16 * tn - 1) / (16 * tn);
-    const dim3 grid((uint32_t)std::min<uint64_t>((waves + 3) / 4, std::max<uint32_t>(1, 4096 / gy)), gy);
-    if (tn == 1) k_linear_narrow<XT, CH, 1><<<grid, 256, 0, st>>>(a, yt);
-    else k_linear_narrow<XT, CH, 4><<<grid, 256, 0, st>>>(a, yt);
-}
-template <int XT> static void linear_narrow(const LinearArgs &a, int yt, hipStream_t st) {
-    if (a.k <= 16) linear_narrow<XT, 1>(a, yt, st);
-    else if (a.k <= 32) linear_narrow<XT, 2>(a, yt, st);
-    else linear_narrow<XT, 4>(a, yt, st);
-}
-
-// ---- few rows: the weights' bytes bound it
-//
-// A block takes 16 channels and all of k, its eight waves 64 of k each in turn, straight from
-// memory into v_mfma_i32_16x16x64_i8 (as above) with MT groups of 16 rows; the waves' sums meet
-// in LDS. FLOATS: up to four rows of floats, quantised by every block into LDS while its first
-// weights are under way (x is small and comes from cache): one launch instead of two.
-constexpr int kFW = 8, kFU = 8;          // waves a block, loads in flight a lane
-constexpr uint32_t kFusedRows = 4, kFusedBytes = 32768;
-
-template <int XT, int MT>
-__global__ __launch_bounds__(64 * kFW) void k_linear_few(LinearArgs a, int yt) {
-    constexpr bool FLOATS = XT != FSX_DTYPE_I8;
-    extern __shared__ __attribute__((aligned(16))) int8_t s_x[];   // FLOATS: the rows' codes, up64(k) + 16 apart
-    __shared__ __attribute__((aligned(16))) v4i s_acc[kFW][MT][64];
-    __shared__ uint32_t s_max[kFusedRows];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
-    const uint64_t n0 = (uint64_t)blockIdx.x * 16, c = n0 + lr < a.n ? n0 + lr : a.n - 1;
-    const uint32_t chunks = (a.k + 63) / 64, pitch = chunks * 64 + 16;
-    const int8_t *pw = a.w + c * a.ldw + 16 * lq;
-    auto weights = [&](uint32_t first, v4i (&w)[kFU]) {
-#pragma unroll
-        for (int u = 0; u < kFU; ++u) {
-            const uint32_t k0 = (first + u * kFW) * 64;
-            w[u] = k0 + 64 <= a.k ? load16(pw + k0, 16) : load16(pw + k0, (int64_t)a.k - k0 - 16 * lq);
-        }
-    };
-    v4i w[kFU];
-    weights(wave, w);
-    if constexpr (FLOATS) {
-        using T = typename Elem<XT>::T;
-        const T *x = static_cast<const T *>(a.x);
-        const uint32_t per = chunks * 4, all = (uint32_t)a.rows * per;   // chunks of 16, zeros behind the end
-        if (threadIdx.x < kFusedRows) s_max[threadIdx.x] = 0;
-        __syncthreads();
-        for (uint32_t q = threadIdx.x; q < all; q += 64 * kFW) {
-            const uint32_t r = q / per, k0 = (q - r * per) * 16;
-            float v[kQV], m = 0.0f;
-            load_row<T, kQV>(x + r * a.ldx + k0, (int64_t)a.k - k0, 0.0f, v);
-#pragma unroll
-            for (int i = 0; i < kQV; ++i) m = amax_of(m, v[i]);
-            // |x| as words are ordered as they are as numbers, NaN above infinity
-            atomicMax(&s_max[r], __float_as_uint(m) & 0x7FFFFFFFu);
-        }
-        __syncthreads();
-        for (uint32_t q = threadIdx.x; q < all; q += 64 * kFW) {
-            const uint32_t r = q / per, k0 = (q - r * per) * 16;
-            float v[kQV];
-            load_row<T, kQV>(x + r * a.ldx + k0, (int64_t)a.k - k0, 0.0f, v);
-            const float s = row_scale(__uint_as_float(s_max[r]));
-            *reinterpret_cast<v4i *>(s_x + r * pitch + k0) = pack_codes(v, 1.0f / s, s, s == s);
-        }
-        __syncthreads();
-    }
-    v4i acc[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[m] = v4i{0, 0, 0, 0};
-    for (uint32_t first = wave; first < chunks; first += kFW * kFU) {
-        if (first != wave) weights(first, w);
-#pragma unroll
-        for (int u = 0; u < kFU; ++u) {
-            const uint32_t k0 = (first + u * kFW) * 64;
-            if (k0 >= a.k) break;
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const uint32_t r = 16 * m + lr, rr = r < a.rows ? r : (uint32_t)a.rows - 1;
-                v4i x;
-                if (FLOATS) x = *reinterpret_cast<const v4i *>(s_x + rr * pitch + k0 + 16 * lq);
-                else x = load16(static_cast<const int8_t *>(a.x) + rr * a.ldx + k0 + 16 * lq,
-                                k0 + 64 <= a.k ? 16 : (int64_t)a.k - k0 - 16 * lq);
-                acc[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u], x, acc[m], 0, 0, 0);
-            }
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m) s_acc[wave][m][lane] = acc[m];
-    __syncthreads();
-    if (wave >= MT) return;
-    v4i sum = s_acc[0][wave][lane];
-#pragma unroll
-    for (int i = 1; i < kFW; ++i) sum += s_acc[i][wave][lane];
-    const uint64_t r = 16 * wave + lr;
-    if (r >= a.rows) return;
-    Channels ch;
-    ch.load(a, n0 + 4 * lq);
-    ch.finish(a, yt, sum, FLOATS ? row_scale(__uint_as_float(s_max[r & (kFusedRows - 1)])) : a.x_scale[r], r,
-              n0 + 4 * lq);
-}
-
-template <int XT> static void linear_few(const LinearArgs &a, int yt, hipStream_t st) {
-    const uint32_t blocks = (a.n + 15) / 16;
-    if constexpr (XT != FSX_DTYPE_I8) {
-        const uint32_t lds = (uint32_t)a.rows * ((a.k + 63) / 64 * 64 + 16);
-        k_linear_few<XT, 1><<<blocks, 64 * kFW, lds, st>>>(a, yt);
-    } else if (a.rows <= 16) k_linear_few<XT, 1><<<blocks, 64 * kFW, 0, st>>>(a, yt);
-    else if (a.rows <= 32) k_linear_few<XT, 2><<<blocks, 64 * kFW, 0, st>>>(a, yt);
-    else k_linear_few<XT, 4><<<blocks, 64 * kFW, 0, st>>>(a, yt);
-}
-
-// ---- tiles of BN channels x BM rows, waves of WN x WM, kBK bytes of k at a time through LDS
+// ---- tiles of BN channels x BM rows, waves of WN x WM, BK bytes of k at a time through LDS
 //
 // The weights are the first operand of v_mfma_i32_32x32x32_i8 and x the second: lane l gives
 // bytes 16 (l / 32) .. of row l % 32 of either, and holds channels 8 j + 4 (l / 32) .. + 3 of
 // row l % 32 of the result: four neighbouring channels of one row.
 //
-// LDS holds a row's kBK bytes as 16-byte chunks, chunk c of row r at place c ^ (r & 7): the
-// eight lanes that read one chunk of eight rows then meet all banks once. Two buffers: while
-// one is multiplied, the next tile's loads fly, one barrier a tile. DMA: the loads write LDS
-// themselves (operands at 16-byte strides); else they pass through registers.
-constexpr int kBK = 128;
+// LDS holds a row's BK bytes as 16-byte chunks, chunk c of row r at place c ^ key(r): sixteen
+// lanes read one chunk of sixteen rows at once, and those of them whose rows share banks (256
+// bytes hold 256 / BK rows) then meet different ones.
+template <int BK> __device__ __forceinline__ uint32_t place_key(uint32_t row) {
+    return row / (256 / BK) % (BK / 16);
+}
 
-template <int ROWS, int THREADS, bool DMA> struct Stage {
-    static constexpr int kLoads = ROWS * kBK / 16 / THREADS;   // chunks a thread brings
-    const int8_t *base;        // the tile's first row
-    uint32_t at, off[kLoads];  // the thread's chunk in a row, and from `base` to its chunks (ld < 2^23)
-    uint64_t row[DMA ? 1 : kLoads];
-    v4i reg[DMA ? 1 : kLoads];
-    // chunk i of this thread: row i * THREADS / 8 + threadIdx / 8, place threadIdx % 8. Rows
-    // behind the last: the last one, its results are not stored.
-    __device__ __forceinline__ void init(const int8_t *p, uint64_t ld, uint64_t r0, uint64_t rows) {
-        const uint32_t tr = threadIdx.x >> 3, pos = threadIdx.x & 7;
-        at = 16 * (pos ^ (tr & 7));
+#ifdef __HIP_DEVICE_COMPILE__   // (buffer descriptors are no host type)
+// A tile's rows of one operand into LDS, LOADS chunks a thread. DMA: the loads write LDS
+// themselves (chunks at 16-byte addresses); else they pass through registers.
+template <int ROWS, int BK, int THREADS, bool DMA> struct Stage {
+    static constexpr int LOADS = ROWS * BK / 16 / THREADS, PER = BK / 16, STEP = THREADS / PER;
+    static_assert(LOADS > 0 && STEP % 16 == 0, "whole rows, the same key for a thread's chunks");
+    const int8_t *base;      // the tile's first row
+    __amdgpu_buffer_rsrc_t buf;   // the tile's rows (DMA): bounds for the hardware
+    uint32_t at, off[LOADS]; // the thread's chunk in a row, and from `base` to its chunks (ld < 2^23)
+    uint64_t row[DMA ? 1 : LOADS];
+    v4i reg[DMA ? 1 : LOADS];
+    // chunk i of this thread: row i STEP + threadIdx / PER, place threadIdx % PER. Rows behind
+    // the last: the last one, its results are not stored.
+    __device__ __forceinline__ void init(const int8_t *p, uint64_t ld, uint64_t r0, uint64_t rows,
+                                         uint32_t k) {
+        const uint32_t tr = threadIdx.x / PER, pos = threadIdx.x % PER;
+        at = 16 * (pos ^ place_key<BK>(tr));
         base = p + r0 * ld;
         const uint32_t last = (uint32_t)(rows - r0 < ROWS ? rows - r0 : ROWS) - 1;
+        // raw buffer, 32-bit data; it ends with the chunk that the last row's end lies in
+        if (DMA) buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(base), 0, last * (uint32_t)ld + ((k + 15) & ~15u), 0x00020000);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const uint32_t r = i * (THREADS / 8) + tr, rr = r < last ? r : last;
+        for (int i = 0; i < LOADS; ++i) {
+            const uint32_t r = i * STEP + tr, rr = r < last ? r : last;
             if (DMA) off[i] = rr * (uint32_t)ld + at;
             else row[i] = rr * ld;
         }
     }
-    // A chunk that starts behind the row's end: the tile's first (x is cleared there); an
+    // A chunk that starts behind the row's end: the row's first (x is cleared there); an
     // aligned chunk that starts inside the row stays in its page.
-    __device__ __forceinline__ void load(int8_t *lds, uint32_t k0, uint32_t k) {
+    __device__ __forceinline__ void load(int8_t *lds, uint32_t wave, uint32_t k0, uint32_t k) {
+        if constexpr (DMA) {
+            auto go = [&](uint32_t back) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            if (DMA) {
-                const int8_t *src = base + k0 + (off[i] - (k0 + at >= k ? at : 0));
-                __builtin_amdgcn_global_load_lds(
-                    (const __attribute__((address_space(1))) void *)src,
-                    (__attribute__((address_space(3))) void *)(lds + (i * THREADS + (threadIdx.x & ~63u)) * 16), 16, 0,
-                    0);
-            } else {
-                reg[i] = load16(base + row[i] + k0 + at, (int64_t)k - k0 - at);
-            }
+                for (int i = 0; i < LOADS; ++i)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                        buf, (__attribute__((address_space(3))) void *)(lds + (i * THREADS + wave * 64) * 16), 16,
+                        off[i] - back, k0, 0, 0);
+            };
+            if (k0 + BK <= k) go(0);
+            else go(k0 + at < k ? 0 : k0 + at);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) reg[i] = load16(base + row[i] + k0 + at, (int64_t)k - k0 - at);
         }
     }
     __device__ __forceinline__ void store(int8_t *lds) {
         if (!DMA)
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i)
+            for (int i = 0; i < LOADS; ++i)
                 *reinterpret_cast<v4i *>(lds + (i * THREADS + threadIdx.x) * 16) = reg[i];
     }
 };
 
-template <int WN, int WM>
+// MF 32: v_mfma_i32_32x32x32_i8, 16: v_mfma_i32_16x16x64_i8.
+template <int MF, int WN, int WM, int BK>
 struct WaveTile {
-    static constexpr int TN = WN / 32, TM = WM / 32, S = kBK / 32;
-    v16i acc[TN][TM];
+    static constexpr int TN = WN / MF, TM = WM / MF, S = BK * MF / 1024, E = MF * MF / 64;
+    typedef int Acc __attribute__((ext_vector_type(E)));
+    Acc acc[TN][TM];
     struct Frag { v4i w[TN], x[TM]; };
-    __device__ __forceinline__ void read(Frag &f, const int8_t *sw, const int8_t *sx, uint32_t wn, uint32_t wm, int s) {
-        const uint32_t lane = __lane_id(), lr = lane & 31, at = ((2 * s + (lane >> 5)) ^ (lr & 7)) * 16;
+    Frag f[2];
+    __device__ __forceinline__ void read(Frag &to, const int8_t *sw, const int8_t *sx, uint32_t wn, uint32_t wm, int s) {
+        const uint32_t lane = __lane_id(), lr = lane % MF, at = ((64 / MF * s + lane / MF) ^ place_key<BK>(lr)) * 16;
 #pragma unroll
-        for (int i = 0; i < TN; ++i) f.w[i] = *reinterpret_cast<const v4i *>(sw + (wn + 32 * i + lr) * kBK + at);
+        for (int i = 0; i < TN; ++i) to.w[i] = *reinterpret_cast<const v4i *>(sw + (wn + MF * i + lr) * BK + at);
 #pragma unroll
-        for (int j = 0; j < TM; ++j) f.x[j] = *reinterpret_cast<const v4i *>(sx + (wm + 32 * j + lr) * kBK + at);
+        for (int j = 0; j < TM; ++j) to.x[j] = *reinterpret_cast<const v4i *>(sx + (wm + MF * j + lr) * BK + at);
     }
-    // One tile of k: a step's reads fly while the step before is multiplied.
-    __device__ __forceinline__ void multiply(const int8_t *sw, const int8_t *sx, uint32_t wn, uint32_t wm) {
-        Frag f[2];
-        read(f[0], sw, sx, wn, wm, 0);
+    // Step s of a tile from f[s & 1], the next step's reads under way meanwhile.
+    template <typename F> __device__ __forceinline__ void step(int s, F next) {
+        __builtin_amdgcn_sched_barrier(0);
+        next(f[(s + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (s + 1 < S) read(f[(s + 1) & 1], sw, sx, wn, wm, s + 1);
+        for (int i = 0; i < TN; ++i)
 #pragma unroll
-            for (int i = 0; i < TN; ++i)
-#pragma unroll
-                for (int j = 0; j < TM; ++j)
+            for (int j = 0; j < TM; ++j) {
+                if constexpr (MF == 32)
                     acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[s & 1].w[i], f[s & 1].x[j], acc[i][j], 0, 0, 0);
-        }
+                else
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s & 1].w[i], f[s & 1].x[j], acc[i][j], 0, 0, 0);
+            }
         __builtin_amdgcn_sched_barrier(0);
     }
 };
 
 // x of the last tile behind the rows' end, `left` bytes into the tile: 0 (weights there count nothing then).
-template <int BM, int THREADS>
+template <int BM, int BK, int THREADS>
 __device__ __forceinline__ void clear_tail(int8_t *sx, uint32_t left) {
-    if (left >= kBK) return;
-    for (uint32_t c = threadIdx.x; c < BM * 8; c += THREADS) {
-        const uint32_t r = c >> 3, first = 16 * ((c & 7) ^ (r & 7));
+    if (left >= BK) return;
+#pragma unroll 1
+    for (uint32_t c = threadIdx.x; c < BM * BK / 16; c += THREADS) {
+        const uint32_t r = c / (BK / 16), first = 16 * (c % (BK / 16) ^ place_key<BK>(r));
         v4i v = *reinterpret_cast<v4i *>(sx + 16 * c);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -504,57 +272,150 @@ __device__ __forceinline__ void clear_tail(int8_t *sx, uint32_t left) {
     __syncthreads();
 }
 
-// What each wave has issued has arrived, its reads too; then all waves are here.
-__device__ __forceinline__ void tile_barrier() {
-    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt 0, lgkmcnt 0
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+// What this wave has issued has arrived but for the last LATER loads, its reads too; then all
+// waves are here.
+template <int LATER> __device__ __forceinline__ void tile_barrier() {
+    __builtin_amdgcn_s_waitcnt((LATER & 15) | (LATER >> 4) << 14 | 0x0070);   // vmcnt LATER, lgkmcnt 0
+    asm volatile("" ::: "memory");        // (no fence: it would wait for the later loads too)
     __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    asm volatile("" ::: "memory");
 }
 
-template <int BN, int BM, int WN, int WM, bool DMA, int YT>
-__global__ __launch_bounds__(BN / WN * (BM / WM) * 64) void k_linear_tile(LinearArgs a, TileGrid tg) {
+#endif
+
+// Two buffers: tile i + 1 is loaded while tile i is multiplied. More (DMA): NS - 1 tiles are
+// under way, the next one is in LDS already and its first step's reads are made ahead of the
+// barrier, so that the matrix instructions go on behind it.
+//
+// Few tiles over a long k: block (.., p) takes bytes p k_part .. of k and leaves its sums in
+// `sums` [p][rows][n]; k_linear_join adds the parts.
+template <int MF, int BN, int BM, int WN, int WM, int BK, int NS, bool DMA, int YT>
+__global__ __launch_bounds__(BN / WN * (BM / WM) * 64) void k_linear_tile(LinearArgs a, TileGrid tg, uint32_t k_part,
+                                                                          int32_t *sums) {
+#ifdef __HIP_DEVICE_COMPILE__
     constexpr int THREADS = BN / WN * (BM / WM) * 64;
-    using T = typename Elem<YT>::T;
-    __shared__ __attribute__((aligned(16))) int8_t s_w0[BN * kBK], s_x0[BM * kBK], s_w1[BN * kBK], s_x1[BM * kBK];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 31, half = lane >> 5;
+    constexpr bool DEEP = NS > 2;
+    static_assert(DMA || !DEEP, "through registers: two buffers");
+    if constexpr (YT == kSums) {
+        const uint32_t from = blockIdx.y * k_part;
+        a.x = static_cast<const int8_t *>(a.x) + from;
+        a.w += from;
+        a.k = a.k - from < k_part ? a.k - from : k_part;
+    }
+    // (a variable for each buffer: the compiler then knows which loads a read has to wait for)
+    constexpr int SIZE = (BN + BM) * BK;
+    __shared__ __attribute__((aligned(16))) int8_t s_0[SIZE], s_1[SIZE], s_2[NS > 2 ? SIZE : 16],
+        s_3[NS > 3 ? SIZE : 16];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane % MF,
+                   part = lane / MF;
     const uint32_t wn = wave % (BN / WN) * WN, wm = wave / (BN / WN) * WM;
     uint32_t bn, bm;
     tg.place(blockIdx.x, bn, bm);
     const uint64_t n0 = (uint64_t)bn * BN, m0 = (uint64_t)bm * BM;
-    WaveTile<WN, WM> t;
+    WaveTile<MF, WN, WM, BK> t;
+    constexpr int S = t.S;
 #pragma unroll
     for (int i = 0; i < t.TN; ++i)
 #pragma unroll
-        for (int j = 0; j < t.TM; ++j) t.acc[i][j] = v16i{};
-    Stage<BN, THREADS, DMA> lw;
-    Stage<BM, THREADS, DMA> lx;
-    lw.init(a.w, a.ldw, n0, a.n);
-    lx.init(static_cast<const int8_t *>(a.x), a.ldx, m0, a.rows);
-    const uint32_t tiles = (a.k + kBK - 1) / kBK;
-    // tile i + 1 into (sw2, sx2) while tile i in (sw, sx) is multiplied
-    auto step = [&](uint32_t i, int8_t *sw, int8_t *sx, int8_t *sw2, int8_t *sx2) {
-        tile_barrier();
-        if (i + 1 < tiles) {
-            lw.load(sw2, (i + 1) * kBK, a.k);
-            lx.load(sx2, (i + 1) * kBK, a.k);
-        } else {
-            clear_tail<BM, THREADS>(sx, a.k - i * kBK);
+        for (int j = 0; j < t.TM; ++j) t.acc[i][j] = {};
+    Stage<BN, BK, THREADS, DMA> lw;
+    Stage<BM, BK, THREADS, DMA> lx;
+    lw.init(a.w, a.ldw, n0, a.n, a.k);
+    lx.init(static_cast<const int8_t *>(a.x), a.ldx, m0, a.rows, a.k);
+    const uint32_t tiles = (a.k + BK - 1) / BK;
+    constexpr int EACH = lw.LOADS + lx.LOADS;
+    auto load = [&](uint32_t i, int8_t *to) {
+        if (i >= tiles) {   // (nothing more to load: no load is under way, so that the count below holds)
+            if (DMA) __builtin_amdgcn_s_waitcnt(0x0F70);
+            return;
         }
-        t.multiply(sw, sx, wn, wm);
-        lw.store(sw2);
-        lx.store(sx2);
+        lw.load(to, wave, i * BK, a.k);
+        lx.load(to + BN * BK, wave, i * BK, a.k);
     };
-    lw.load(s_w0, 0, a.k);
-    lx.load(s_x0, 0, a.k);
-    lw.store(s_w0);
-    lx.store(s_x0);
-    for (uint32_t i = 0; i < tiles; i += 2) {
-        step(i, s_w0, s_x0, s_w1, s_x1);
-        if (i + 1 < tiles) step(i + 1, s_w1, s_x1, s_w0, s_x0);
+    auto read = [&](typename WaveTile<MF, WN, WM, BK>::Frag &to, const int8_t *from, int s) {
+        t.read(to, from, from + BN * BK, wn, wm, s);
+    };
+    auto tail = [&](uint32_t i, int8_t *of) {
+        if (i + 1 == tiles) clear_tail<BM, BK, THREADS>(of + BN * BK, a.k - i * BK);
+    };
+    auto multiply = [&](const int8_t *from, auto last) {   // last(f): the reads beside the last step
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            t.step(s, [&](auto &f) {
+                if (s + 1 < S) read(f, from, s + 1);
+                else last(f);
+            });
+    };
+    load(0, s_0);
+    if constexpr (!DEEP) {
+        lw.store(s_0);
+        lx.store(s_0 + BN * BK);
+        auto step = [&](uint32_t i, int8_t *from, int8_t *to) {
+            tile_barrier<0>();
+            tail(i, from);
+            read(t.f[0], from, 0);
+            load(i + 1, to);
+            multiply(from, [](auto &) {});
+            lw.store(to);
+            lx.store(to + BN * BK);
+        };
+        for (uint32_t i = 0;;) {
+            step(i, s_0, s_1);
+            if (++i == tiles) break;
+            step(i, s_1, s_0);
+            if (++i == tiles) break;
+        }
+    } else {
+        static_assert(S % 2 == 0, "a tile's first step is in f[0]");
+        load(1, s_1);
+        if constexpr (NS > 3) load(2, s_2);
+        tile_barrier<(NS - 2) * EACH>();
+        tail(0, s_0);
+        read(t.f[0], s_0, 0);
+        // tile i from `from`; tile i + 1 has arrived in `next`, tile i + NS - 1 goes to `to`, which
+        // held tile i - 1
+        auto step = [&](uint32_t i, int8_t *from, int8_t *next, int8_t *to) {
+            tile_barrier<(NS - 3) * EACH>();
+            tail(i + 1, next);
+            load(i + NS - 1, to);
+            multiply(from, [&](auto &f) { read(f, next, 0); });   // (behind the last tile: unused)
+        };
+        for (uint32_t i = 0;;) {
+            if constexpr (NS == 3) {
+                step(i, s_0, s_1, s_2);
+                if (++i == tiles) break;
+                step(i, s_1, s_2, s_0);
+                if (++i == tiles) break;
+                step(i, s_2, s_0, s_1);
+                if (++i == tiles) break;
+            } else {
+                step(i, s_0, s_1, s_3);
+                if (++i == tiles) break;
+                step(i, s_1, s_2, s_0);
+                if (++i == tiles) break;
+                step(i, s_2, s_3, s_1);
+                if (++i == tiles) break;
+                step(i, s_3, s_0, s_2);
+                if (++i == tiles) break;
+            }
+        }
     }
+    if constexpr (YT == kSums) {
+#pragma unroll
+        for (int i = 0; i < t.TN; ++i)
+#pragma unroll
+            for (int j = 0; j < t.TM; ++j) {
+                const uint64_t r = m0 + wm + MF * j + lr, c = n0 + wn + MF * i + 4 * part;
+                if (r >= a.rows) continue;
+                int32_t *to = sums + (blockIdx.y * a.rows + r) * a.n;
+#pragma unroll
+                for (int e = 0; e < t.E; ++e)
+                    if (c + 8 * (e / 4) + e % 4 < a.n) to[c + 8 * (e / 4) + e % 4] = t.acc[i][j][e];
+            }
+    } else {
+    using T = typename Elem<YT>::T;
     // the channels' scales and biases come through LDS
-    float *s_ws = reinterpret_cast<float *>(s_w0), *s_b = reinterpret_cast<float *>(s_w1);
+    float *s_ws = reinterpret_cast<float *>(s_0), *s_b = s_ws + BN;
     __syncthreads();
     for (uint32_t c = threadIdx.x; c < BN; c += THREADS) {
         const uint64_t cc = n0 + c < a.n ? n0 + c : a.n - 1;
@@ -564,81 +425,144 @@ __global__ __launch_bounds__(BN / WN * (BM / WM) * 64) void k_linear_tile(Linear
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < t.TN; ++i) {
-        const uint32_t cw = wn + 32 * i + 4 * half;
+        const uint32_t cw = wn + MF * i + 4 * part;
         const int64_t left = (int64_t)a.n - (int64_t)(n0 + cw);   // channels from this lane's first on
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < t.TM; ++j) {
-            const uint64_t r = m0 + wm + 32 * j + lr;
+            const uint64_t r = m0 + wm + MF * j + lr;
             const float xs = a.x_scale[r < a.rows ? r : a.rows - 1];
-            float v[16];
+            float v[t.E / 4][4];
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                v[e] = scaled(t.acc[i][j][e], xs, s_ws[cw + 8 * (e / 4) + e % 4], s_b[cw + 8 * (e / 4) + e % 4]);
-            if (a.act == FSX_ACT_RELU) {
+            for (int e = 0; e < t.E; ++e)
+                v[e / 4][e % 4] = scaled(t.acc[i][j][e], xs, s_ws[cw + 8 * (e / 4) + e % 4], s_b[cw + 8 * (e / 4) + e % 4]);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = relu(v[e]);
-            } else if (a.act == FSX_ACT_SIGMOID) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = sigmoid(v[e]);
-            }
+            for (int g = 0; g < t.E / 4; ++g) activate(v[g], a.act);
             if (r >= a.rows) continue;
             T *y = static_cast<T *>(a.y) + r * a.ldy + n0 + cw;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float o[4] = {v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
-                if (left > 8 * g) store4(y + 8 * g, o, left - 8 * g);
-            }
+            for (int g = 0; g < t.E / 4; ++g)
+                if (left > 8 * g) store4(y + 8 * g, v[g], left - 8 * g);
         }
+    }
+    }
+#endif
+}
+
+// The parts' sums, four channels of a row a thread.
+__global__ __launch_bounds__(256) void k_linear_join(LinearArgs a, int yt, uint32_t parts, const int32_t *sums) {
+    const uint32_t per = (a.n + 3) / 4;
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < a.rows * per; i += gridDim.x * 256ull) {
+        const uint64_t r = i / per;
+        const uint32_t c = (uint32_t)(i - r * per) * 4;
+        v4i sum = {0, 0, 0, 0};
+#pragma unroll 8
+        for (uint32_t p = 0; p < parts; ++p) {
+            const int32_t *from = sums + (p * a.rows + r) * a.n + c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += from[c + e < a.n ? e : 0];
+        }
+        put_sums(a, yt, sum, a.x_scale[r], r, c);
     }
 }
 
-template <int BN, int BM, int WN, int WM, bool DMA>
+// Rows that the DMA cannot bring into rows that it can, 16 bytes a thread; 0 behind their ends.
+__global__ __launch_bounds__(256) void k_pack_rows(const int8_t *p, uint64_t ld, uint64_t rows, uint32_t k, int8_t *to) {
+    const uint32_t per = (k + 15) / 16;
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < rows * per; i += gridDim.x * 256ull) {
+        const uint64_t r = i / per;
+        const uint32_t c = (uint32_t)(i - r * per) * 16;
+        *reinterpret_cast<v4i *>(to + 16 * i) = load16(p + r * ld + c, (int64_t)k - c);
+    }
+}
+
+template <int MF, int BN, int BM, int WN, int WM, int BK, int NS, bool DMA>
 static void linear_tile(const LinearArgs &a, int yt, hipStream_t st) {
     const TileGrid tg((a.n + BN - 1) / BN, (a.rows + BM - 1) / BM);
     constexpr int threads = BN / WN * (BM / WM) * 64;
-    if (yt == FSX_DTYPE_F32) k_linear_tile<BN, BM, WN, WM, DMA, FSX_DTYPE_F32><<<tg.tiles, threads, 0, st>>>(a, tg);
-    else if (yt == FSX_DTYPE_F16) k_linear_tile<BN, BM, WN, WM, DMA, FSX_DTYPE_F16><<<tg.tiles, threads, 0, st>>>(a, tg);
-    else k_linear_tile<BN, BM, WN, WM, DMA, FSX_DTYPE_BF16><<<tg.tiles, threads, 0, st>>>(a, tg);
+    auto go = [&](auto kernel) { kernel<<<tg.tiles, threads, 0, st>>>(a, tg, a.k, nullptr); };
+    if (yt == FSX_DTYPE_F32) go(k_linear_tile<MF, BN, BM, WN, WM, BK, NS, DMA, FSX_DTYPE_F32>);
+    else if (yt == FSX_DTYPE_F16) go(k_linear_tile<MF, BN, BM, WN, WM, BK, NS, DMA, FSX_DTYPE_F16>);
+    else go(k_linear_tile<MF, BN, BM, WN, WM, BK, NS, DMA, FSX_DTYPE_BF16>);
 }
 
 // Operands that the DMA can bring: chunks at 16-byte addresses, a tile's rows within 2^31 bytes.
 static bool dma_can(const void *p, uint64_t ld) { return ((uintptr_t)p | ld) % 16 == 0 && ld < (1u << 23); }
 
-static void linear_tiles(const LinearArgs &a, int yt, hipStream_t st) {
-    const bool dma = dma_can(a.x, a.ldx) && dma_can(a.w, a.ldw);
-    auto tiles = [&](uint64_t bn, uint64_t bm) { return (a.n + bn - 1) / bn * ((a.rows + bm - 1) / bm); };
-    if (tiles(256, 256) >= 256) {
-        if (dma) linear_tile<256, 256, 128, 64, true>(a, yt, st);
-        else linear_tile<256, 256, 128, 64, false>(a, yt, st);
-    } else if (tiles(128, 128) >= 256) {
-        if (dma) linear_tile<128, 128, 64, 64, true>(a, yt, st);
-        else linear_tile<128, 128, 64, 64, false>(a, yt, st);
-    } else {
-        if (dma) linear_tile<64, 64, 32, 32, true>(a, yt, st);
-        else linear_tile<64, 64, 32, 32, false>(a, yt, st);
-    }
-}
-
-// Which form takes a product, by its sizes and x's type alone.
+// How a product goes, by its sizes, x's type and whether the DMA can bring x and the weights.
+//
+// kNarrow: fsx_narrow.hip. kFewFloats, kFew: k_linear_few, for codes up to 32 rows (us at 16 / 32
+// rows of 4096 to 4096 channels: 6.7 / 8.7, in tiles 9.8 / 10.8; to 16384 channels 20.7 / 28, in
+// tiles 14.9 / 15.5, since those fill the CUs).
+// kTiles: k_linear_tile. With few tiles over a long k in parts: enough blocks for the CUs, each
+// with 1024 of k at least (223 rows of 3777 to 14 channels 23.8 -> 12.4 us). With many, operands
+// that the DMA cannot bring are packed first (4096 rows of 4096 to 4096 channels at odd strides:
+// 155 us through registers).
 enum LinearForm { kNarrow, kFewFloats, kFew, kTiles };
-static LinearForm form_of(uint64_t rows, uint32_t k, int x_dtype) {
-    if (k <= 64) return kNarrow;
-    if (x_dtype != FSX_DTYPE_I8 && rows <= kFusedRows && rows * ((k + 63) / 64 * 64 + 16) <= kFusedBytes)
-        return kFewFloats;
-    return rows <= 64 ? kFew : kTiles;
-}
+struct LinearPlan {
+    LinearForm form;
+    uint32_t parts = 1, k_part = 0;
+    bool pack_x = false, pack_w = false;
+    uint64_t codes = 0, x_bytes = 0, w_bytes = 0, sums = 0;   // of the workspace, in this order
+    uint64_t bytes() const { return codes + x_bytes + w_bytes + sums; }
 
-uint64_t linear_work(uint64_t rows, uint32_t k, uint32_t n, int x_dtype) {
-    (void)n;
-    const LinearForm f = form_of(rows, k, x_dtype);
-    return x_dtype == FSX_DTYPE_I8 || f == kNarrow || f == kFewFloats ? 0 : code_space(rows, k).bytes;
+    LinearPlan(uint64_t rows, uint32_t k, uint32_t n, int x_dtype, bool x_fits, bool w_fits) {
+        const bool floats = x_dtype != FSX_DTYPE_I8;
+        auto tiles = [&](uint64_t size) { return (n + size - 1) / size * ((rows + size - 1) / size); };
+        if (k <= 64) form = kNarrow;
+        else if (floats && rows <= kFusedRows && rows * ((k + 63) / 64 * 64 + 16) <= kFusedBytes) form = kFewFloats;
+        else if ((rows <= 16 && n < 16384 && (k < 16384 || n >= 2048)) || (rows <= 32 && n < 8192 && k < 8192))
+            form = kFew;
+        else form = kTiles;
+        if (floats && (form == kFew || form == kTiles)) codes = code_space(rows, k).bytes;
+        if (form != kTiles) return;
+        if (tiles(64) < 128 && k >= 2048) {
+            const uint32_t want = (uint32_t)std::min<uint64_t>({256 / tiles(64), k / 1024, 64});
+            k_part = ((k + want - 1) / want + 255) / 256 * 256;
+            parts = (k + k_part - 1) / k_part;
+            if (parts > 1) sums = up16(parts * rows * n * 4);
+        } else if (tiles(128) >= 256) {
+            pack_x = !floats && !x_fits;
+            pack_w = !w_fits;
+            if (pack_x) x_bytes = rows * up16(k);
+            if (pack_w) w_bytes = n * up16(k);
+        }
+    }
+};
+
+// Large tiles read least for each product; with fewer of them than the CUs, smaller ones. us at
+// 512 / 1024 / 2048 / 4096 rows of 4096 to 4096 channels:
+//                      256 x 256     54    55    57    70    (8192 cubed: 507)
+//   128 x 128, two buffers           26    28    37    71-77 (572)
+//   128 x 128, four buffers          23    25    55    95    (one block a CU)
+//    64 x 64                         16    33    64   119    (909)
+// Eight waves a block in each: four waves of twice the size were 12 - 60 % slower, since a wave
+// by itself issues an instruction in 8 cycles.
+static void linear_tiles(const LinearArgs &a, int yt, const LinearPlan &ks, void *sums_at, hipStream_t st) {
+    if (ks.parts > 1) {
+        const TileGrid tg((a.n + 63) / 64, (a.rows + 63) / 64);
+        const dim3 grid(tg.tiles, ks.parts);
+        int32_t *sums = static_cast<int32_t *>(sums_at);
+        if (dma_can(a.x, a.ldx) && dma_can(a.w, a.ldw))
+            k_linear_tile<16, 64, 64, 32, 16, 256, 2, true, kSums><<<grid, 512, 0, st>>>(a, tg, ks.k_part, sums);
+        else k_linear_tile<16, 64, 64, 32, 16, 128, 2, false, kSums><<<grid, 512, 0, st>>>(a, tg, ks.k_part, sums);
+        const uint64_t blocks = (a.rows * ((a.n + 3) / 4) + 255) / 256;
+        k_linear_join<<<(uint32_t)std::min<uint64_t>(blocks, 4096), 256, 0, st>>>(a, yt, ks.parts, sums);
+        return;
+    }
+    auto tiles = [&](uint64_t size) { return (a.n + size - 1) / size * ((a.rows + size - 1) / size); };
+    if (dma_can(a.x, a.ldx) && dma_can(a.w, a.ldw)) {
+        if (tiles(256) >= 256) linear_tile<16, 256, 256, 128, 64, 128, 2, true>(a, yt, st);
+        else if (tiles(128) >= 320) linear_tile<16, 128, 128, 64, 32, 128, 2, true>(a, yt, st);
+        else if (tiles(128) >= 192) linear_tile<16, 128, 128, 64, 32, 128, 4, true>(a, yt, st);
+        else linear_tile<16, 64, 64, 32, 16, 256, 2, true>(a, yt, st);
+    } else linear_tile<16, 64, 64, 32, 16, 128, 2, false>(a, yt, st);
 }
 
 // A grid holds fewer than 2^32 threads: a product beyond 2^20 channels, or of more results than
 // 2^38, goes out in several launches.
 template <typename F>
-static void slabs(const LinearArgs &a, int y_dtype, F launch, uint32_t x_size = 1) {
+static void slabs(const LinearArgs &a, int y_dtype, uint32_t x_size, F launch) {
     const uint64_t most_n = 1ull << 20;
     for (uint64_t n0 = 0; n0 < a.n; n0 += most_n) {
         const uint64_t n = std::min<uint64_t>(a.n - n0, most_n);
@@ -658,38 +582,58 @@ static void slabs(const LinearArgs &a, int y_dtype, F launch, uint32_t x_size = 
     }
 }
 
-template <int XT> static void linear_floats(const LinearArgs &a, LinearForm f, int yt, hipStream_t st) {
-    if (f == kNarrow) linear_narrow<XT>(a, yt, st);
-    else linear_few<XT>(a, yt, st);
+// (what a call needs; any x of codes: as if its rows were at odd strides)
+uint64_t linear_work(uint64_t rows, uint32_t k, uint32_t n, int x_dtype, const void *x, uint64_t ldx, const void *w,
+                     uint64_t ldw) {
+    return LinearPlan(rows, k, n, x_dtype, x && dma_can(x, ldx), dma_can(w, ldw)).bytes();
+}
+
+static void pack_rows(const int8_t *p, uint64_t ld, uint64_t rows, uint32_t k, int8_t *to, hipStream_t st) {
+    const uint64_t blocks = (rows * ((k + 15) / 16) + 255) / 256;
+    k_pack_rows<<<(uint32_t)std::min<uint64_t>(blocks, 8192), 256, 0, st>>>(p, ld, rows, k, to);
 }
 
 hipError_t launch_linear(const LinearArgs &in, int x_dtype, int y_dtype, void *work, hipStream_t st) {
     (void)hipGetLastError();
     if (in.rows == 0 || in.n == 0) return hipSuccess;
-    const LinearForm f = form_of(in.rows, in.k, x_dtype);
     LinearArgs a = in;
+    const LinearPlan p(a.rows, a.k, a.n, x_dtype, dma_can(a.x, a.ldx), dma_can(a.w, a.ldw));
+    if (x_dtype != FSX_DTYPE_I8 && (p.form == kNarrow || p.form == kFewFloats)) {
+        slabs(a, y_dtype, elem_size(x_dtype), [&](const LinearArgs &b) {
+            if (p.form == kNarrow) launch_linear_narrow(b, x_dtype, y_dtype, st);
+            else if (x_dtype == FSX_DTYPE_F32) linear_few<FSX_DTYPE_F32>(b, y_dtype, st);
+            else if (x_dtype == FSX_DTYPE_F16) linear_few<FSX_DTYPE_F16>(b, y_dtype, st);
+            else linear_few<FSX_DTYPE_BF16>(b, y_dtype, st);
+        });
+        return hipGetLastError();
+    }
+    int8_t *at = static_cast<int8_t *>(work);
     if (x_dtype != FSX_DTYPE_I8) {
-        if (f == kNarrow || f == kFewFloats) {
-            slabs(a, y_dtype, [&](const LinearArgs &b) {
-                if (x_dtype == FSX_DTYPE_F32) linear_floats<FSX_DTYPE_F32>(b, f, y_dtype, st);
-                else if (x_dtype == FSX_DTYPE_F16) linear_floats<FSX_DTYPE_F16>(b, f, y_dtype, st);
-                else linear_floats<FSX_DTYPE_BF16>(b, f, y_dtype, st);
-            }, elem_size(x_dtype));
-            return hipGetLastError();
-        }
         const CodeSpace s = code_space(a.rows, a.k);
-        int8_t *q = static_cast<int8_t *>(work);
-        float *sc = reinterpret_cast<float *>(q + s.scale_at);
-        const hipError_t e = launch_quantize_rows(a.x, x_dtype, a.rows, a.k, a.ldx, q, s.ld, sc, st);
+        float *sc = reinterpret_cast<float *>(at + s.scale_at);
+        const hipError_t e = launch_quantize_rows(a.x, x_dtype, a.rows, a.k, a.ldx, at, s.ld, sc, st);
         if (e != hipSuccess) return e;
-        a.x = q;
+        a.x = at;
         a.x_scale = sc;
         a.ldx = s.ld;
+        at += p.codes;
     }
-    slabs(a, y_dtype, [&](const LinearArgs &b) {
-        if (f == kNarrow) linear_narrow<FSX_DTYPE_I8>(b, y_dtype, st);
-        else if (f == kFew) linear_few<FSX_DTYPE_I8>(b, y_dtype, st);
-        else linear_tiles(b, y_dtype, st);
+    if (p.pack_x) {
+        pack_rows(static_cast<const int8_t *>(a.x), a.ldx, a.rows, a.k, at, st);
+        a.x = at;
+        a.ldx = up16(a.k);
+        at += p.x_bytes;
+    }
+    if (p.pack_w) {
+        pack_rows(a.w, a.ldw, a.n, a.k, at, st);
+        a.w = at;
+        a.ldw = up16(a.k);
+        at += p.w_bytes;
+    }
+    slabs(a, y_dtype, 1, [&](const LinearArgs &b) {
+        if (p.form == kNarrow) launch_linear_narrow(b, FSX_DTYPE_I8, y_dtype, st);
+        else if (p.form == kFew) linear_few<FSX_DTYPE_I8>(b, y_dtype, st);
+        else linear_tiles(b, y_dtype, p, at, st);   // (in parts: small enough for one launch)
     });
     return hipGetLastError();
 }

@@ -15,35 +15,6 @@ namespace fsx {
 constexpr float kLowest = -3.402823466e38f;   // the maximum of no values: finite, so that -inf - m is -inf
 constexpr float kLog2e = 1.4426950408889634f;
 
-// The value of lane ^ O, without LDS where the hardware has a lane permutation for it.
-template <int O> __device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
-    static_assert(O == 1 || O == 2 || O == 4 || O == 8 || O == 16 || O == 32, "one bit");
-    if constexpr (O == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);          // quad_perm 1 0 3 2
-    else if constexpr (O == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);     // quad_perm 2 3 0 1
-    else if constexpr (O == 4) return __builtin_amdgcn_ds_swizzle(v, 0x101F);                // xor 4
-    else if constexpr (O == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, true);    // row_ror 8
-    else if constexpr (O == 16) return __builtin_amdgcn_ds_swizzle(v, 0x401F);               // xor 16
-    else {
-        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-        return __lane_id() < 32 ? r[1] : r[0];
-    }
-}
-template <int O> __device__ __forceinline__ float xor_lane(float v) {
-    return __uint_as_float(xor_lane<O>(__float_as_uint(v)));
-}
-template <int O> __device__ __forceinline__ unsigned long long xor_lane(unsigned long long v) {
-    return (unsigned long long)xor_lane<O>((uint32_t)(v >> 32)) << 32 | xor_lane<O>((uint32_t)v);
-}
-// f over the G lanes (a power of two) of a group, in every lane of it
-template <int G, typename T, typename F> __device__ __forceinline__ T group_all(T v, F f) {
-    if constexpr (G > 1) v = f(v, xor_lane<1>(v));
-    if constexpr (G > 2) v = f(v, xor_lane<2>(v));
-    if constexpr (G > 4) v = f(v, xor_lane<4>(v));
-    if constexpr (G > 8) v = f(v, xor_lane<8>(v));
-    if constexpr (G > 16) v = f(v, xor_lane<16>(v));
-    if constexpr (G > 32) v = f(v, xor_lane<32>(v));
-    return v;
-}
 struct Larger { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
 struct LargerFloat { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
 struct Plus { __device__ float operator()(float a, float b) const { return a + b; } };

@@ -1,0 +1,104 @@
+// fsx_quantize.hip — rows of floats to int8 codes with one scale a row (include/fsx_hip.h
+// fsx_quantize_rows_device): scale_r = max(fl32(max_c |x_rc| / 127), 2^-126),
+// q_rc = x_rc / scale_r to the nearest whole number, halves to even.
+#include <hip/hip_runtime.h>
+#include <algorithm>
+
+#include "fsx_q8_rows.h"
+
+namespace fsx {
+
+// A group of TPR threads takes a row, up to C chunks of kQV values a thread; they stay in
+// registers between the maximum and the codes (C 0: longer rows are read twice, the second
+// time from cache).
+template <int DT, int TPR, int C>
+__global__ __launch_bounds__(256) void k_quantize_rows(const void *__restrict__ xp, uint64_t rows, uint32_t cols,
+                                                       uint64_t ldx, int8_t *__restrict__ q, uint64_t ldq,
+                                                       float *__restrict__ scale) {
+    using T = typename Elem<DT>::T;
+    constexpr uint32_t RPB = 256 / TPR, STEP = TPR * kQV;
+    __shared__ uint32_t s_max[4];
+    const uint32_t t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    for (uint64_t r0 = (uint64_t)blockIdx.x * RPB; r0 < rows; r0 += (uint64_t)gridDim.x * RPB) {
+        const uint64_t r = r0 + sub;
+        const bool live = r < rows;
+        const T *x = static_cast<const T *>(xp) + (live ? r : 0) * ldx;
+        uint32_t m = 0;
+        RawChunk<DT> kept[C ? C : 1];
+        if constexpr (C > 0) {
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const uint32_t c = t * kQV + i * STEP;
+                if (live && c < cols) kept[i].load(x + c, (int64_t)cols - c);
+            }
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (live && t * kQV + i * STEP < cols) m = max(m, kept[i].mag());
+        } else if (live) {
+            for (uint64_t c = t * kQV; c < cols; c += STEP) {
+                kept[0].load(x + c, (int64_t)cols - (int64_t)c);
+                m = max(m, kept[0].mag());
+            }
+        }
+        m = group_all<TPR < 64 ? TPR : 64>(m, LargerWord());
+        if constexpr (TPR > 64) {
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
+            __syncthreads();
+            m = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+        }
+        if (!live) continue;
+        const float s = row_scale(mag_value<DT>(m));
+        const bool ok = s == s;
+        const float inv = 1.0f / s;
+        if (t == 0) scale[r] = s;
+        int8_t *qr = q + r * ldq;
+        auto put = [&](uint32_t c, const RawChunk<DT> &k) {
+            const v4i o = ok ? k.codes(inv, s) : v4i{0, 0, 0, 0};
+            if (cols - c >= kQV) __builtin_memcpy(qr + c, &o, kQV);
+            else
+#pragma unroll
+                for (int i = 0; i < kQV; ++i) if (c + i < cols) qr[c + i] = (int8_t)(o[i / 4] >> (8 * (i % 4)));
+        };
+        if constexpr (C > 0) {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (t * kQV + i * STEP < cols) put(t * kQV + i * STEP, kept[i]);
+        } else {
+            for (uint64_t c = t * kQV; c < cols; c += STEP) {
+                kept[0].load(x + c, (int64_t)cols - (int64_t)c);
+                put((uint32_t)c, kept[0]);
+            }
+        }
+    }
+}
+
+template <int DT>
+static void quantize_rows(const void *x, uint64_t rows, uint32_t cols, uint64_t ldx, int8_t *q, uint64_t ldq,
+                          float *scale, hipStream_t st) {
+    const uint32_t per = (cols + kQV - 1) / kQV;   // chunks of a row
+    auto go = [&](auto kernel, uint32_t tpr) {
+        const uint64_t blocks = (rows + 256 / tpr - 1) / (256 / tpr);
+        kernel<<<(uint32_t)std::min<uint64_t>(blocks, 1u << 16), 256, 0, st>>>(x, rows, cols, ldx, q, ldq, scale);
+    };
+    if (per <= 1) go(k_quantize_rows<DT, 1, 1>, 1);
+    else if (per <= 4) go(k_quantize_rows<DT, 4, 1>, 4);
+    else if (per <= 16) go(k_quantize_rows<DT, 16, 1>, 16);
+    else if (per <= 64) go(k_quantize_rows<DT, 64, 1>, 64);
+    else if (per <= 256) go(k_quantize_rows<DT, 256, 1>, 256);
+    else if (per <= 512) go(k_quantize_rows<DT, 256, 2>, 256);
+    else if (per <= 1024) go(k_quantize_rows<DT, 256, 4>, 256);
+    else go(k_quantize_rows<DT, 256, 0>, 256);
+}
+
+hipError_t launch_quantize_rows(const void *x, int dtype, uint64_t rows, uint32_t cols, uint64_t ldx, int8_t *q,
+                                uint64_t ldq, float *scale, hipStream_t st) {
+    (void)hipGetLastError();
+    if (rows == 0) return hipSuccess;
+    if (dtype == FSX_DTYPE_F32) quantize_rows<FSX_DTYPE_F32>(x, rows, cols, ldx, q, ldq, scale, st);
+    else if (dtype == FSX_DTYPE_F16) quantize_rows<FSX_DTYPE_F16>(x, rows, cols, ldx, q, ldq, scale, st);
+    else quantize_rows<FSX_DTYPE_BF16>(x, rows, cols, ldx, q, ldq, scale, st);
+    return hipGetLastError();
+}
+
+}  // namespace fsx
