@@ -582,10 +582,10 @@ static void slabs(const LinearArgs &a, int y_dtype, uint32_t x_size, F launch) {
     }
 }
 
-// (what a call needs; any x of codes: as if its rows were at odd strides)
+// What a call needs; without a pointer: as if those rows were at odd strides.
 uint64_t linear_work(uint64_t rows, uint32_t k, uint32_t n, int x_dtype, const void *x, uint64_t ldx, const void *w,
                      uint64_t ldw) {
-    return LinearPlan(rows, k, n, x_dtype, x && dma_can(x, ldx), dma_can(w, ldw)).bytes();
+    return LinearPlan(rows, k, n, x_dtype, x && dma_can(x, ldx), w && dma_can(w, ldw)).bytes();
 }
 
 static void pack_rows(const int8_t *p, uint64_t ld, uint64_t rows, uint32_t k, int8_t *to, hipStream_t st) {

@@ -330,7 +330,9 @@ int fsx_quantize_rows_device(fsx_ctx *ctx, const void *d_x, int x_dtype, size_t 
  * rounded once to y's type; the sum is exact (int32). RELU keeps NaN; SIGMOID is
  * 1 / (1 + e^-v). x is either codes (FSX_DTYPE_I8) with their row scales d_x_scale, or floats
  * (d_x_scale NULL) whose rows are quantised within the call as fsx_quantize_rows_device does.
- * 1 <= in_features <= 131071 (the sum of any int8 codes then fits in 32 bits). */
+ * 1 <= in_features <= 131071 (the sum of any int8 codes then fits in 32 bits). Codes and
+ * weights may lie anywhere; large products are fastest with both at 16-byte addresses and
+ * strides (ld a multiple of 16), others are first copied to such places in the workspace. */
 #define FSX_ACT_NONE 0
 #define FSX_ACT_RELU 1
 #define FSX_ACT_SIGMOID 2
@@ -344,8 +346,12 @@ typedef struct fsx_q8_linear {
     int32_t activation;          /* FSX_ACT_* */
     uint32_t reserved;           /* 0 */
 } fsx_q8_linear;
-/* Workspace bytes of the call below (0: none needed; host only). Quantised rows live there,
- * and the partial sums of products with few rows. 0 for arguments that the call refuses. */
+/* Workspace bytes of the call below (0: none needed; host only), 0 for arguments that the call
+ * refuses. Quantised rows live there, the partial sums of small products over long rows, and
+ * the copies of operands of large products that are not at 16-byte addresses and strides: the
+ * weights' are known from the layer (a null weight counts as not), codes x as if they were not
+ * (the call itself then needs less). It is the size for this number of rows: fewer rows may
+ * need more, so a program with batches of several sizes takes the largest of their sizes. */
 size_t fsx_linear_q8_work(const fsx_q8_linear *layer, int x_dtype, size_t rows);
 int fsx_linear_q8_device(fsx_ctx *ctx, const fsx_q8_linear *layer, const void *d_x, int x_dtype, size_t ldx,
                          const float *d_x_scale, size_t rows, void *d_y, int y_dtype, size_t ldy,

@@ -247,6 +247,109 @@ def test_linear_garbage_behind_rows(head):
             check_linear(head, x, None, w, ws, None, "none", torch.float32)
 
 
+# (rows, k, n, bytes between rows of x, of the weights): strides of 16 bytes or not, one tile of
+# k or several with a rest, a last tile of a few rows and channels
+TILES = [(4097, 130, 4000, 14, 14), (4097, 70, 4000, 10, 10), (2300, 100, 2305, 12, 12), (2300, 300, 2305, 4, 4),
+         (1700, 70, 1801, 10, 10), (1700, 200, 1801, 8, 8), (1700, 390, 1801, 10, 10), (1700, 700, 1801, 4, 4),
+         (300, 65, 400, 15, 15), (300, 520, 400, 8, 8), (300, 65, 400, 0, 15), (300, 777, 403, 0, 0),
+         (2100, 333, 2100, 0, 0), (2100, 333, 2100, 3, 0), (2100, 333, 2100, 0, 3), (4100, 65, 4100, 1, 2),
+         (100, 5000, 200, 8, 8), (100, 5001, 200, 0, 0), (17, 2048, 100, 0, 0), (40, 2049, 7, 15, 15), (40, 2049, 7, 0, 15),
+         (33, 131071, 65, 1, 1), (20, 4096, 16390, 0, 0), (2, 16400, 100, 0, 0), (16, 9000, 2050, 8, 8),
+         (9, 9001, 130, 0, 0), (16, 300, 9000, 4, 4), (31, 300, 8000, 4, 5)]
+
+
+@pytest.mark.parametrize("rows,k,n,xpad,wpad", TILES)
+def test_linear_forms(head, rows, k, n, xpad, wpad):
+    """Each way that a product of codes takes through the GPU, in a workspace of exactly its size."""
+    g = gen_of("tiles", rows, k, n, xpad, wpad)
+    w, ws, bias = layer_of(g, n, k, wpad, True)
+    x = codes_of(g, rows, k, xpad)
+    xs = (0.005 + 0.01 * torch.rand(rows, generator=g)).cuda()
+    layer = head.layer(w, ws, bias, "none")
+    need = head.lib.linear_q8_work(layer, head.lib.DTYPE_I8, rows)
+    work = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
+    y = torch.full((rows + 1, n + 3), float(CANARY), device="cuda")
+    torch.cuda.synchronize()
+    head.linear(layer, x, xs, y[:rows, :n], work[:need])
+    torch.cuda.synchronize()
+    assert (work[need:] == 255).all(), "behind the workspace"
+    assert (y[rows] == CANARY).all() and (y[:, n:] == CANARY).all(), "what is behind the rows was written"
+    ref, tol = head_ref.linear(x.cpu().long(), xs, w, ws, bias, "none", torch.float32)
+    head_ref.assert_close(y[:rows, :n], ref, tol, "y")
+
+
+def test_linear_forms_agree(head):
+    """A row's results have the same bits in any batch, at any stride, from codes or floats."""
+    g = gen_of("agree")
+    for k, n, most in ((4096, 520, 700), (500, 2100, 2100), (60, 33, 300)):
+        w, ws, bias = layer_of(g, n, k, 0, True)
+        odd = codes_of(g, n, k, 3)
+        odd.copy_(w)
+        x = rows_of(g, most, k, 0, torch.bfloat16)
+        q, s = torch.empty(most, k, dtype=torch.int8, device="cuda"), torch.empty(most, device="cuda")
+        torch.cuda.synchronize()
+        head.quantize(x, q, s)
+        whole = None
+        for weight in (w, odd):
+            layer = head.layer(weight, ws, bias, "sigmoid")
+            for rows in (most, 300, 33, 17, 5, 4, 1):
+                for xx, xs in ((x[:rows], None), (q[:rows], s)):
+                    y = torch.empty(rows, n, device="cuda")
+                    work = head.linear_work(layer, xx)
+                    torch.cuda.synchronize()
+                    head.linear(layer, xx, xs, y, work)
+                    torch.cuda.synchronize()
+                    whole = y if whole is None else whole
+                    assert torch.equal(y, whole[:rows]), (k, n, rows)
+
+
+@pytest.mark.parametrize("rows,k,n,xpad,wpad", [(100, 5000, 200, 8, 8), (2100, 333, 2100, 0, 0), (1700, 390, 1801, 10, 10)])
+def test_linear_forms_replayed(head, rows, k, n, xpad, wpad):
+    """Products in parts and with copied operands, captured and replayed on other codes."""
+    g = gen_of("replay", rows)
+    w, ws, bias = layer_of(g, n, k, wpad, True)
+    x = codes_of(g, rows, k, xpad)
+    xs = torch.rand(rows, generator=g).cuda()
+    y = torch.empty(rows, n, dtype=torch.bfloat16, device="cuda")
+    layer = head.layer(w, ws, bias, "relu")
+    work = head.linear_work(layer, x)
+    torch.cuda.synchronize()
+    head.linear(layer, x, xs, y, work)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=head.stream):
+        head.linear(layer, x, xs, y, work)
+    for _ in range(4):
+        x.copy_(codes_of(g, rows, k, 0))
+        w.copy_(codes_of(g, n, k, 0))
+        work.fill_(255)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = y.clone()
+        y.zero_()
+        torch.cuda.synchronize()
+        head.linear(layer, x, xs, y, work)
+        torch.cuda.synchronize()
+        assert torch.equal(got, y)
+
+
+@pytest.mark.parametrize("xt", FLOATS)
+@pytest.mark.parametrize("rows,k", [(4, 8176), (4, 8177), (3, 10000), (2, 16368), (1, 32752), (1, 32753), (4, 65), (1, 16385)])
+def test_linear_floats_few(head, xt, rows, k):
+    """Floats quantised by every block, up to the LDS they may fill, and the sizes behind it."""
+    g = gen_of("ff", rows, k)
+    w, ws, bias = layer_of(g, 37, k, 3, True)
+    check_linear(head, rows_of(g, rows, k, 1, FLOATS[xt]), None, w, ws, bias, "none", torch.float32)
+
+
+def test_linear_floats_few_many_channels(head):
+    """.. with eight waves a block instead of sixteen."""
+    g = gen_of("ffn")
+    w, ws, bias = layer_of(g, 8200, 300, 4, True)
+    check_linear(head, rows_of(g, 3, 300, 1, torch.float16), None, w, ws, bias, "none", torch.float32)
+
+
 def test_linear_far_rows(head):
     """x, weights and y beyond 2^31 elements from their first."""
     g = gen_of("far")
@@ -375,6 +478,24 @@ def test_logprobs_special_rows(head, dtype, classes):
     x[16] = 1e-30
     x[17, classes - 1] = 60000.0
     check_logprobs(head, x.to(t), top=min(33, 2 * classes))
+
+
+@pytest.mark.parametrize("rows,classes,top", [(1030, 1500, 64), (1030, 5003, 1), (1030, 2048, 33), (30, 9000, 64),
+                                              (3, 200001, 64), (3, 60000, 1), (257, 20000, 32)])
+def test_logprobs_orders(head, rows, classes, top):
+    """Rows whose candidates outrun any bound: rising, equal, falling, all of a few values."""
+    g = gen_of("orders", rows, classes)
+    x = 3 * torch.randn(rows, classes, generator=g)
+    step = torch.arange(classes) / classes
+    x[0] = step * 9
+    x[1] = 2.5
+    if rows > 2: x[2] = -step * 9
+    if rows > 3:
+        x[3] = torch.randint(0, 3, (classes,), generator=g).float()
+        x[4] = (torch.arange(classes) // 512 % 7).float()
+        x[rows - 1] = step * 3
+        x[rows - 2, 1:] = NEG
+    check_logprobs(head, x.cuda(), top=top)
 
 
 def test_logprobs_parts(head):

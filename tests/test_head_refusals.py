@@ -84,6 +84,13 @@ def test_linear_workspace(fake, native):
     assert native.load_library().fsx_linear_q8_work(None, 0, 8) == 0
 
 
+def test_linear_workspace_before_the_weights(fake, native):
+    """A program may ask before its weights are there: then the size covers any place of theirs."""
+    for rows, k, n, ld in ((5000, 512, 5000, 512), (5000, 500, 5000, 500), (100, 4096, 64, 4096), (2, 9, 5, 9)):
+        sizes = [native.linear_q8_work(native.q8_linear(w, P, None, k, n, ld), native.DTYPE_I8, rows) for w in (P, P + 1, None)]
+        assert sizes[2] == max(sizes), (rows, k, n, ld)
+
+
 def logp(fake, work=0, work_bytes=0, **over):
     a = dict(x=P, dtype=0, rows=4, classes=50, ld=50, target=P, logprob=P, entropy=P, top=3, ids=P, lps=P)
     a.update(over)
