@@ -5,6 +5,7 @@
 //   y_rn    = act((float)(sum_k q_rk w_nk) * scale_r * t_n + b_n)
 #include <hip/hip_runtime.h>
 #include <algorithm>
+#include <type_traits>
 
 #include "fsx_q8_rows.h"
 
@@ -14,44 +15,71 @@ constexpr int kSums = -1;   // results that are sums still
 
 // ---------------------------------------------------------------- int8 product
 
-// ---- few rows: the weights' bytes bound it
+// ---- few rows or few channels: the longer side's bytes bound it
 //
-// A block takes 16 channels and all of k, its FW waves 128 bytes of k (whole lines) each in turn,
-// straight from memory into v_mfma_i32_16x16x64_i8, the weights first: lane l gives bytes
-// 16 (l / 16) .. of row l % 16 of either operand and holds channels 4 (l / 16) .. of row l % 16
-// of the result. MT groups of 16 rows; the waves' sums meet in LDS. FLOATS: up to four rows of
-// floats, quantised by every block into LDS while its first weights are under way (x is small
-// and comes from cache): one launch instead of two.
-constexpr int kFU = 8;          // loads of weights in flight a lane
-constexpr uint32_t kFusedRows = 4, kFusedBytes = 32768;
+// The longer side is the rows of x (TALL) or the channels; the other one has up to 32, MT groups
+// of 16. A block takes 16 of the longer side for each `kw` of its FW waves, which share its k 128
+// bytes (whole lines) in turn, straight from memory into v_mfma_i32_16x16x64_i8, the weights
+// first: lane l gives bytes 16 (l / 16) .. of row l % 16 of either operand and holds channels
+// 4 (l / 16) .. of row l % 16 of the result. The waves' sums meet in LDS. Few blocks over a long
+// k: block (.., p) takes bytes p k_part .. of k, and k_linear_join adds the parts.
+//
+// FLOATS: a block quantises its rows of x into LDS, in one launch with the product: all rows if
+// they are few (every block does, while its first weights are under way; x is small and comes
+// from cache), else (TALL) its own.
+constexpr uint32_t kDirectMost = 32, kFusedRows = 4, kFusedBytes = 32768, kTallBytes = 49152;
 
-template <int XT, int MT, int FW>
-__global__ __launch_bounds__(64 * FW) void k_linear_few(LinearArgs a, int yt) {
+template <int XT, int MT, int FW, bool TALL, bool ODD>
+__global__ __launch_bounds__(64 * FW) void k_linear_direct(LinearArgs a, int yt, uint32_t kw, uint32_t k_part,
+                                                           int32_t *sums) {
     constexpr bool FLOATS = XT != FSX_DTYPE_I8;
     constexpr uint32_t THREADS = 64 * FW;
+    constexpr int U = MT == 1 && !TALL ? 8 : 4;   // loads of the longer side in flight a lane
     extern __shared__ __attribute__((aligned(16))) int8_t s_x[];   // FLOATS: the rows' codes, up64(k) + 16 apart
     __shared__ __attribute__((aligned(16))) v4i s_acc[FW][MT][64];
-    __shared__ uint32_t s_max[kFusedRows];
+    __shared__ uint32_t s_max[TALL ? 16 * FW : kFusedRows];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15,
                    lq = lane >> 4;
-    const uint64_t n0 = (uint64_t)blockIdx.x * 16, c = n0 + lr < a.n ? n0 + lr : a.n - 1;
+    const uint32_t groups = FW / kw, wk = wave % kw, group = wave / kw;   // (kw divides FW)
+    const uint64_t longer = TALL ? a.rows : a.n, shorter = TALL ? a.n : a.rows;
+    const uint64_t l0 = (uint64_t)blockIdx.x * groups * 16;   // the block's first
+    const uint32_t from = blockIdx.y * k_part, end = a.k - from < k_part ? a.k : from + k_part;
     const uint32_t chunks = (a.k + 63) / 64, pitch = chunks * 64 + 16;
-    const int8_t *pw = a.w + c * a.ldw + 16 * lq;
-    // the wave's u-th load of round t: the place in k of 64 bytes
-    auto place = [&](uint32_t t, int u) { return (2 * (wave + FW * (t * (kFU / 2) + u / 2)) + u % 2) * 64; };
-    auto load = [&](const int8_t *p, uint32_t k0) {
-        return k0 + 64 <= a.k ? load16(p + k0, 16) : load16(p + k0, (int64_t)a.k - k0 - 16 * lq);
-    };
-    v4i w[kFU];
-    auto weights = [&](uint32_t t) {
+    const uint64_t mine = l0 + 16 * group + lr, l = mine < longer ? mine : longer - 1;
+    const int8_t *pl = (TALL ? static_cast<const int8_t *>(a.x) + (FLOATS ? 0 : l * a.ldx) : a.w + l * a.ldw) + 16 * lq;
+    const int8_t *ps[MT];
 #pragma unroll
-        for (int u = 0; u < kFU; ++u) w[u] = load(pw, place(t, u));
+    for (int m = 0; m < MT; ++m) {
+        const uint64_t r = 16 * m + lr, rr = r < shorter ? r : shorter - 1;
+        ps[m] = (TALL ? a.w + rr * a.ldw : static_cast<const int8_t *>(a.x) + (FLOATS ? 0 : rr * a.ldx)) + 16 * lq;
+    }
+    // The wave's u-th block of round t, of `whole` blocks of 64 bytes and then a rest.
+    const uint32_t whole = (end - from) / 64;
+    auto block = [&](uint32_t t, int u) { return 2 * (wk + kw * (t * (U / 2) + u / 2)) + u % 2; };
+    auto place = [&](uint32_t i) { return from + i * 64; };
+    auto code = [&](uint32_t r, uint32_t k0) {   // FLOATS: of row r in LDS
+        return *reinterpret_cast<const v4i *>(s_x + r * pitch + k0 + 16 * lq);
     };
-    weights(0);
+    auto lds_row = [&](int m) -> uint32_t {
+        const uint32_t r = 16 * m + lr;
+        return TALL ? 16 * group + lr : r < a.rows ? r : (uint32_t)a.rows - 1;
+    };
+    constexpr bool AHEAD = !(FLOATS && TALL);   // (those come from LDS)
+    v4i v[U];
+    auto longs = [&](uint32_t t) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (block(t, u) < whole)
+                v[u] = AHEAD ? load16_at(pl + place(block(t, u)), ODD) : code(lds_row(0), place(block(t, u)));
+    };
+    if (AHEAD && block(0, 0) < whole) longs(0);
     if constexpr (FLOATS) {
-        const auto *x = static_cast<const typename Elem<XT>::T *>(a.x);
-        const uint32_t per = chunks * 4, all = (uint32_t)a.rows * per;   // chunks of 16, zeros behind the end
-        if (threadIdx.x < kFusedRows) s_max[threadIdx.x] = 0;
+        const uint64_t r0 = TALL ? l0 : 0;
+        const uint32_t most = TALL ? groups * 16 : (uint32_t)a.rows;
+        const uint32_t rows = a.rows - r0 < most ? (uint32_t)(a.rows - r0) : most;
+        const auto *x = static_cast<const typename Elem<XT>::T *>(a.x) + r0 * a.ldx;
+        const uint32_t per = chunks * 4, all = rows * per;   // chunks of 16, zeros behind the end
+        for (uint32_t i = threadIdx.x; i < most; i += THREADS) s_max[i] = 0;
         __syncthreads();
         RawChunk<XT> first;   // (kept: rows of up to 16 THREADS values are read once)
         auto each = [&](auto f) {
@@ -68,10 +96,10 @@ __global__ __launch_bounds__(64 * FW) void k_linear_few(LinearArgs a, int yt) {
                 m = raw.mag();
             }
             if (q0 == 0) first = raw;
-            const uint32_t r0 = __builtin_amdgcn_readfirstlane(r);
-            if (__ballot(some && r != r0) == 0) {
+            const uint32_t r1 = __builtin_amdgcn_readfirstlane(r);
+            if (__ballot(some && r != r1) == 0) {
                 m = group_all<64>(m, LargerWord());
-                if (lane == 0) atomicMax(&s_max[r0], m);
+                if (lane == 0) atomicMax(&s_max[r1], m);
             } else if (some) {
                 atomicMax(&s_max[r], m);
             }
@@ -92,49 +120,109 @@ __global__ __launch_bounds__(64 * FW) void k_linear_few(LinearArgs a, int yt) {
     v4i acc[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[m] = v4i{0, 0, 0, 0};
-    for (uint32_t t = 0; place(t, 0) < a.k; ++t) {
-        if (t) weights(t);
+    auto multiply = [&](int m, const v4i &of_long, const v4i &of_short) {
+        acc[m] = TALL ? __builtin_amdgcn_mfma_i32_16x16x64_i8(of_short, of_long, acc[m], 0, 0, 0)
+                      : __builtin_amdgcn_mfma_i32_16x16x64_i8(of_long, of_short, acc[m], 0, 0, 0);
+    };
+#pragma unroll 1
+    for (uint32_t t = 0; block(t, 0) < whole; ++t) {
+        if (!AHEAD) longs(t);
+        v4i w[MT][U];
 #pragma unroll
-        for (int u = 0; u < kFU; ++u) {
-            const uint32_t k0 = place(t, u);
-            if (k0 >= a.k) break;
+        for (int u = 0; u < U; ++u) {
+            if (block(t, u) >= whole) continue;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const uint32_t r = 16 * m + lr, rr = r < a.rows ? r : (uint32_t)a.rows - 1;
-                v4i x;
-                if (FLOATS) x = *reinterpret_cast<const v4i *>(s_x + rr * pitch + k0 + 16 * lq);
-                else x = load(static_cast<const int8_t *>(a.x) + rr * a.ldx + 16 * lq, k0);
-                acc[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u], x, acc[m], 0, 0, 0);
-            }
+            for (int m = 0; m < MT; ++m)
+                w[m][u] = FLOATS && !TALL ? code(lds_row(m), place(block(t, u))) : load16_at(ps[m] + place(block(t, u)), ODD);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (block(t, u) >= whole) continue;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) multiply(m, v[u], w[m][u]);
+        }
+        if (AHEAD && block(t + 1, 0) < whole) longs(t + 1);
+    }
+    if (end % 64 && wk == whole / 2 % kw) {   // the rest, by the wave whose turn it is (`from` is a multiple of 64)
+        const uint32_t k0 = from + whole * 64;
+        const int ok = (int)(end - k0) - (int)(16 * lq);
+        const v4i rest = AHEAD ? load16_end(pl + k0, ok) : code(lds_row(0), k0);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+            multiply(m, rest, FLOATS && !TALL ? code(lds_row(m), k0) : load16_end(ps[m] + k0, ok));
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) s_acc[wave][m][lane] = acc[m];
     __syncthreads();
-    if (wave >= MT) return;
-    v4i sum = s_acc[0][wave][lane];
+    for (uint32_t i = wave; i < groups * MT; i += FW) {
+        const uint32_t g = i / MT, m = i % MT;
+        v4i sum = s_acc[g * kw][m][lane];
+        for (uint32_t q = 1; q < kw; ++q) sum += s_acc[g * kw + q][m][lane];
+        const uint64_t r = (TALL ? l0 + 16 * g : 16 * m) + lr, c = (TALL ? 16 * m : l0 + 16 * g) + 4 * lq;
+        if (r >= a.rows) continue;
+        if (!FLOATS && sums) {
+            int32_t *to = sums + (blockIdx.y * a.rows + r) * a.n + c;
 #pragma unroll
-    for (int i = 1; i < FW; ++i) sum += s_acc[i][wave][lane];
-    const uint64_t r = 16 * wave + lr;
-    if (r >= a.rows) return;
-    float xs;
-    if constexpr (FLOATS) xs = row_scale(mag_value<XT>(s_max[r]));
-    else xs = a.x_scale[r];
-    put_sums(a, yt, sum, xs, r, n0 + 4 * lq);
+            for (int e = 0; e < 4; ++e)
+                if (c + e < a.n) to[e] = sum[e];
+            continue;
+        }
+        float xs;
+        if constexpr (FLOATS) xs = row_scale(mag_value<XT>(s_max[TALL ? 16 * g + lr : r]));
+        else xs = a.x_scale[r];
+        put_sums(a, yt, sum, xs, r, c);
+    }
 }
 
-template <int XT, int MT> static void linear_few(const LinearArgs &a, uint32_t lds, int yt, hipStream_t st) {
-    const uint32_t blocks = (a.n + 15) / 16;
-    // us of one row, 4096 / 8192 / 16384 channels of 4096: eight waves 6.4 / 9.1 / 16.8, sixteen
-    // 5.9 / 10.9 / 20.0
-    if (blocks >= 512) k_linear_few<XT, MT, 8><<<blocks, 512, lds, st>>>(a, yt);
-    else k_linear_few<XT, MT, 16><<<blocks, 1024, lds, st>>>(a, yt);
+// The shape of such a product's launch.
+struct DirectGrid {
+    bool tall;
+    uint32_t waves, kw, blocks;
+    static uint64_t pitch(uint32_t k) { return (k + 63) / 64 * 64 + 16; }
+    DirectGrid(uint64_t rows, uint32_t k, uint32_t n, bool floats) {
+        tall = n <= rows && !(floats && rows <= kFusedRows);
+        const uint64_t sixteens = ((tall ? rows : n) + 15) / 16;
+        // us of one row, 4096 / 8192 / 16384 channels of 4096: eight waves 6.4 / 9.1 / 16.8, sixteen
+        // 5.9 / 10.9 / 20.0
+        waves = sixteens >= 512 ? 8 : 16;
+        // (256 bytes of k a wave at least, if the blocks are enough without the others)
+        kw = waves;
+        while (kw > 1 && k < 256 * kw && sixteens * kw / waves >= 512 &&
+               !(floats && tall && waves / kw * 2 * 16 * pitch(k) > kFusedBytes))
+            kw /= 2;
+        blocks = (uint32_t)((sixteens * kw + waves - 1) / waves);
+    }
+    uint64_t codes_bytes(uint64_t rows, uint32_t k) const { return pitch(k) * (tall ? waves / kw * 16 : rows); }
+};
+template <int XT, int MT, bool TALL>
+static void linear_direct(const LinearArgs &a, const DirectGrid &d, uint32_t lds, uint32_t parts, uint32_t k_part,
+                          int32_t *sums, int yt, hipStream_t st) {
+    const bool odd = (((uintptr_t)a.w | a.ldw) & 3) || (XT == FSX_DTYPE_I8 && (((uintptr_t)a.x | a.ldx) & 3));
+    auto go = [&](auto kernel) {
+        kernel<<<dim3(d.blocks, parts), 64 * d.waves, lds, st>>>(a, yt, d.kw, k_part, sums);
+    };
+    if (d.waves == 8) odd ? go(k_linear_direct<XT, MT, 8, TALL, true>) : go(k_linear_direct<XT, MT, 8, TALL, false>);
+    else odd ? go(k_linear_direct<XT, MT, 16, TALL, true>) : go(k_linear_direct<XT, MT, 16, TALL, false>);
 }
-template <int XT> static void linear_few(const LinearArgs &a, int yt, hipStream_t st) {
-    if constexpr (XT != FSX_DTYPE_I8)
-        linear_few<XT, 1>(a, (uint32_t)a.rows * ((a.k + 63) / 64 * 64 + 16), yt, st);
-    else if (a.rows <= 16) linear_few<XT, 1>(a, 0, yt, st);
-    else linear_few<XT, 2>(a, 0, yt, st);
+template <int XT>
+static void linear_direct(const LinearArgs &a, uint32_t parts, uint32_t k_part, int32_t *sums, int yt, hipStream_t st) {
+    constexpr bool FLOATS = XT != FSX_DTYPE_I8;
+    const DirectGrid d(a.rows, a.k, a.n, FLOATS);
+    const uint32_t groups = (uint32_t)(((d.tall ? a.n : a.rows) + 15) / 16);
+    const uint32_t lds = FLOATS ? (uint32_t)d.codes_bytes(a.rows, a.k) : 0;
+    auto go = [&](auto mt, auto tall) {
+        linear_direct<XT, mt, tall>(a, d, lds, parts, k_part, sums, yt, st);
+    };
+    using std::integral_constant;
+    if (d.tall) {
+        if (groups == 1) go(integral_constant<int, 1>(), std::true_type());
+        else go(integral_constant<int, 2>(), std::true_type());
+    } else if constexpr (FLOATS) {
+        go(integral_constant<int, 1>(), std::false_type());
+    } else {
+        if (groups == 1) go(integral_constant<int, 1>(), std::false_type());
+        else go(integral_constant<int, 2>(), std::false_type());
+    }
 }
 
 // The tiles of a product over the launch's blocks. Blocks go to the 8 XCDs in turn, each with
@@ -177,6 +265,7 @@ template <int ROWS, int BK, int THREADS, bool DMA> struct Stage {
     __amdgpu_buffer_rsrc_t buf;   // the tile's rows (DMA): bounds for the hardware
     uint32_t at, off[LOADS]; // the thread's chunk in a row, and from `base` to its chunks (ld < 2^23)
     uint64_t row[DMA ? 1 : LOADS];
+    bool odd;                // strides that are no multiple of 4
     v4i reg[DMA ? 1 : LOADS];
     // chunk i of this thread: row i STEP + threadIdx / PER, place threadIdx % PER. Rows behind
     // the last: the last one, its results are not stored.
@@ -185,6 +274,7 @@ template <int ROWS, int BK, int THREADS, bool DMA> struct Stage {
         const uint32_t tr = threadIdx.x / PER, pos = threadIdx.x % PER;
         at = 16 * (pos ^ place_key<BK>(tr));
         base = p + r0 * ld;
+        odd = (((uintptr_t)p | ld) & 3) != 0;
         const uint32_t last = (uint32_t)(rows - r0 < ROWS ? rows - r0 : ROWS) - 1;
         // raw buffer, 32-bit data; it ends with the chunk that the last row's end lies in
         if (DMA) buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(base), 0, last * (uint32_t)ld + ((k + 15) & ~15u), 0x00020000);
@@ -210,7 +300,10 @@ template <int ROWS, int BK, int THREADS, bool DMA> struct Stage {
             else go(k0 + at < k ? 0 : k0 + at);
         } else {
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) reg[i] = load16(base + row[i] + k0 + at, (int64_t)k - k0 - at);
+            for (int i = 0; i < LOADS; ++i) {
+                const int8_t *p = base + row[i] + k0 + at;
+                reg[i] = k0 + BK <= k ? load16_at(p, odd) : load16_end(p, (int)(k - k0) - (int)at);
+            }
         }
     }
     __device__ __forceinline__ void store(int8_t *lds) {
@@ -466,13 +559,20 @@ __global__ __launch_bounds__(256) void k_linear_join(LinearArgs a, int yt, uint3
     }
 }
 
+static void join_parts(const LinearArgs &a, int yt, uint32_t parts, const int32_t *sums, hipStream_t st) {
+    const uint64_t blocks = (a.rows * ((a.n + 3) / 4) + 255) / 256;
+    k_linear_join<<<(uint32_t)std::min<uint64_t>(blocks, 4096), 256, 0, st>>>(a, yt, parts, sums);
+}
+
 // Rows that the DMA cannot bring into rows that it can, 16 bytes a thread; 0 behind their ends.
 __global__ __launch_bounds__(256) void k_pack_rows(const int8_t *p, uint64_t ld, uint64_t rows, uint32_t k, int8_t *to) {
     const uint32_t per = (k + 15) / 16;
+    const bool odd = (((uintptr_t)p | ld) & 3) != 0;
     for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < rows * per; i += gridDim.x * 256ull) {
         const uint64_t r = i / per;
         const uint32_t c = (uint32_t)(i - r * per) * 16;
-        *reinterpret_cast<v4i *>(to + 16 * i) = load16(p + r * ld + c, (int64_t)k - c);
+        const int8_t *from = p + r * ld + c;
+        *reinterpret_cast<v4i *>(to + 16 * i) = c + 16 <= k ? load16_at(from, odd) : load16_end(from, (int)(k - c));
     }
 }
 
@@ -491,42 +591,68 @@ static bool dma_can(const void *p, uint64_t ld) { return ((uintptr_t)p | ld) % 1
 
 // How a product goes, by its sizes, x's type and whether the DMA can bring x and the weights.
 //
-// kNarrow: fsx_narrow.hip. kFewFloats, kFew: k_linear_few, for codes up to 32 rows (us at 16 / 32
-// rows of 4096 to 4096 channels: 6.7 / 8.7, in tiles 9.8 / 10.8; to 16384 channels 20.7 / 28, in
-// tiles 14.9 / 15.5, since those fill the CUs).
-// kTiles: k_linear_tile. With few tiles over a long k in parts: enough blocks for the CUs, each
-// with 1024 of k at least (223 rows of 3777 to 14 channels 23.8 -> 12.4 us). With many, operands
-// that the DMA cannot bring are packed first (4096 rows of 4096 to 4096 channels at odd strides:
-// 155 us through registers).
-enum LinearForm { kNarrow, kFewFloats, kFew, kTiles };
+// kNarrow: fsx_narrow.hip. kDirectFloats, kDirect: k_linear_direct, up to 32 rows or channels. It
+// takes the shorter side's bytes once for every 16 of the longer one, so large weights are better
+// in tiles, that fill the CUs then (us at 1 / 16 / 32 rows of 4096, direct and in tiles: 4096
+// channels 6.0 / 7.2 / 9.5 and 9.5 / 9.8 / 10.8, 16384 channels 17.1 / 20.5 / 27.6 and 14.8 / 14.9 /
+// 15.5; weights at odd strides, which tiles take through registers, to 16384 channels 19.5 / 29.6
+// and 28.2 / 28.4). Few channels, 2^20 rows of 1024 to 16: 277, in tiles 317.
+// kTiles: k_linear_tile.
+//
+// Few blocks over a long k are cut into parts; the join is another launch. In tiles: 40 rows of
+// 10931 to 42 channels 14.3 us in 10 parts, 13.3 in 20. Direct: 14 rows of 11313 to 1384 channels
+// 24 -> 12.8, but one row of 4096 to 1024 channels 4.8 -> 7.1: by the bytes that a block takes.
+// Operands that the DMA cannot bring are packed for it where the work repays the copy: 4096 rows
+// of 4096 to 4096 channels at odd strides 182 -> 78 us, 1006 rows of 8444 to 2643 channels 104 ->
+// 64, but 1000 rows of 1003 to 777 channels 8.0 -> 12.2.
+enum LinearForm { kNarrow, kDirectFloats, kDirect, kTiles };
 struct LinearPlan {
     LinearForm form;
-    uint32_t parts = 1, k_part = 0;
+    uint32_t parts = 1, k_part;
     bool pack_x = false, pack_w = false;
     uint64_t codes = 0, x_bytes = 0, w_bytes = 0, sums = 0;   // of the workspace, in this order
     uint64_t bytes() const { return codes + x_bytes + w_bytes + sums; }
 
-    LinearPlan(uint64_t rows, uint32_t k, uint32_t n, int x_dtype, bool x_fits, bool w_fits) {
+    LinearPlan(uint64_t rows, uint32_t k, uint32_t n, int x_dtype, bool x_fits, bool w_fits) : k_part(k) {
         const bool floats = x_dtype != FSX_DTYPE_I8;
-        auto tiles = [&](uint64_t size) { return (n + size - 1) / size * ((rows + size - 1) / size); };
-        if (k <= 64) form = kNarrow;
-        else if (floats && rows <= kFusedRows && rows * ((k + 63) / 64 * 64 + 16) <= kFusedBytes) form = kFewFloats;
-        else if ((rows <= 16 && n < 16384 && (k < 16384 || n >= 2048)) || (rows <= 32 && n < 8192 && k < 8192))
-            form = kFew;
-        else form = kTiles;
-        if (floats && (form == kFew || form == kTiles)) codes = code_space(rows, k).bytes;
-        if (form != kTiles) return;
-        if (tiles(64) < 128 && k >= 2048) {
-            const uint32_t want = (uint32_t)std::min<uint64_t>({256 / tiles(64), k / 1024, 64});
+        auto cut = [&](uint64_t blocks, uint32_t enough, uint32_t least) {
+            const uint32_t want = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({enough / blocks, k / least, 64}));
             k_part = ((k + want - 1) / want + 255) / 256 * 256;
             parts = (k + k_part - 1) / k_part;
             if (parts > 1) sums = up16(parts * rows * n * 4);
-        } else if (tiles(128) >= 256) {
-            pack_x = !floats && !x_fits;
+            else k_part = k;
+        };
+        if (k <= 64) {
+            form = kNarrow;
+            return;
+        }
+        if (floats) {
+            const DirectGrid d(rows, k, n, true);
+            const uint64_t lds = d.codes_bytes(rows, k);
+            if (d.tall ? n <= kDirectMost && lds <= kTallBytes : rows <= kFusedRows && lds <= kFusedBytes) {
+                form = kDirectFloats;
+                return;
+            }
+            codes = code_space(rows, k).bytes;
+            x_fits = true;   // (what the quantiser leaves)
+        }
+        const DirectGrid d(rows, k, n, false);
+        const uint64_t shorter = d.tall ? n : rows, weights = (uint64_t)n * k;
+        if (shorter <= kDirectMost && (d.tall || (shorter <= 16 ? weights < 1u << 26 || !w_fits : weights < 1u << 25))) {
+            form = kDirect;
+            const uint64_t taken = (shorter <= 16 ? 32 : 48) * (uint64_t)k * (x_fits && w_fits ? 1 : 2);
+            if (d.blocks <= 128 && taken >= 400000) cut(d.blocks, 256, 1024);
+            return;
+        }
+        form = kTiles;
+        if ((double)rows * n * k >= 2.5e9 && (w_fits || rows >= 384) && (x_fits || n >= 384)) {
+            pack_x = !x_fits;
             pack_w = !w_fits;
             if (pack_x) x_bytes = rows * up16(k);
             if (pack_w) w_bytes = n * up16(k);
         }
+        const uint64_t tiles = (n + 63ull) / 64 * ((rows + 63) / 64);
+        if (tiles < 128 && k >= 2048) cut(tiles, 512, 512);
     }
 };
 
@@ -546,8 +672,7 @@ static void linear_tiles(const LinearArgs &a, int yt, const LinearPlan &ks, void
         if (dma_can(a.x, a.ldx) && dma_can(a.w, a.ldw))
             k_linear_tile<16, 64, 64, 32, 16, 256, 2, true, kSums><<<grid, 512, 0, st>>>(a, tg, ks.k_part, sums);
         else k_linear_tile<16, 64, 64, 32, 16, 128, 2, false, kSums><<<grid, 512, 0, st>>>(a, tg, ks.k_part, sums);
-        const uint64_t blocks = (a.rows * ((a.n + 3) / 4) + 255) / 256;
-        k_linear_join<<<(uint32_t)std::min<uint64_t>(blocks, 4096), 256, 0, st>>>(a, yt, ks.parts, sums);
+        join_parts(a, yt, ks.parts, sums, st);
         return;
     }
     auto tiles = [&](uint64_t size) { return (a.n + size - 1) / size * ((a.rows + size - 1) / size); };
@@ -556,17 +681,19 @@ static void linear_tiles(const LinearArgs &a, int yt, const LinearPlan &ks, void
         else if (tiles(128) >= 320) linear_tile<16, 128, 128, 64, 32, 128, 2, true>(a, yt, st);
         else if (tiles(128) >= 192) linear_tile<16, 128, 128, 64, 32, 128, 4, true>(a, yt, st);
         else linear_tile<16, 64, 64, 32, 16, 256, 2, true>(a, yt, st);
-    } else linear_tile<16, 64, 64, 32, 16, 128, 2, false>(a, yt, st);
+    } else {
+        linear_tile<16, 64, 64, 32, 16, 128, 2, false>(a, yt, st);
+    }
 }
 
 // A grid holds fewer than 2^32 threads: a product beyond 2^20 channels, or of more results than
-// 2^38, goes out in several launches.
+// 2^34, goes out in several launches.
 template <typename F>
 static void slabs(const LinearArgs &a, int y_dtype, uint32_t x_size, F launch) {
     const uint64_t most_n = 1ull << 20;
     for (uint64_t n0 = 0; n0 < a.n; n0 += most_n) {
         const uint64_t n = std::min<uint64_t>(a.n - n0, most_n);
-        const uint64_t most_m = (1ull << 38) / std::max<uint64_t>(n, 1024);
+        const uint64_t most_m = (1ull << 34) / std::max<uint64_t>(n, 1024);
         for (uint64_t m0 = 0; m0 < a.rows; m0 += most_m) {
             LinearArgs b = a;
             b.n = (uint32_t)n;
@@ -598,12 +725,12 @@ hipError_t launch_linear(const LinearArgs &in, int x_dtype, int y_dtype, void *w
     if (in.rows == 0 || in.n == 0) return hipSuccess;
     LinearArgs a = in;
     const LinearPlan p(a.rows, a.k, a.n, x_dtype, dma_can(a.x, a.ldx), dma_can(a.w, a.ldw));
-    if (x_dtype != FSX_DTYPE_I8 && (p.form == kNarrow || p.form == kFewFloats)) {
+    if (x_dtype != FSX_DTYPE_I8 && (p.form == kNarrow || p.form == kDirectFloats)) {
         slabs(a, y_dtype, elem_size(x_dtype), [&](const LinearArgs &b) {
             if (p.form == kNarrow) launch_linear_narrow(b, x_dtype, y_dtype, st);
-            else if (x_dtype == FSX_DTYPE_F32) linear_few<FSX_DTYPE_F32>(b, y_dtype, st);
-            else if (x_dtype == FSX_DTYPE_F16) linear_few<FSX_DTYPE_F16>(b, y_dtype, st);
-            else linear_few<FSX_DTYPE_BF16>(b, y_dtype, st);
+            else if (x_dtype == FSX_DTYPE_F32) linear_direct<FSX_DTYPE_F32>(b, 1, b.k, nullptr, y_dtype, st);
+            else if (x_dtype == FSX_DTYPE_F16) linear_direct<FSX_DTYPE_F16>(b, 1, b.k, nullptr, y_dtype, st);
+            else linear_direct<FSX_DTYPE_BF16>(b, 1, b.k, nullptr, y_dtype, st);
         });
         return hipGetLastError();
     }
@@ -632,7 +759,11 @@ hipError_t launch_linear(const LinearArgs &in, int x_dtype, int y_dtype, void *w
     }
     slabs(a, y_dtype, 1, [&](const LinearArgs &b) {
         if (p.form == kNarrow) launch_linear_narrow(b, FSX_DTYPE_I8, y_dtype, st);
-        else if (p.form == kFew) linear_few<FSX_DTYPE_I8>(b, y_dtype, st);
+        else if (p.form == kDirect) {
+            int32_t *sums = p.parts > 1 ? reinterpret_cast<int32_t *>(at) : nullptr;
+            linear_direct<FSX_DTYPE_I8>(b, p.parts, p.k_part, sums, y_dtype, st);
+            if (sums) join_parts(b, y_dtype, p.parts, sums, st);
+        }
         else linear_tiles(b, y_dtype, p, at, st);   // (in parts: small enough for one launch)
     });
     return hipGetLastError();

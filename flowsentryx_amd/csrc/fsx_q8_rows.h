@@ -155,6 +155,47 @@ __device__ __forceinline__ v4i load16(const int8_t *p, int64_t ok) {
     return v;
 }
 
+// 16 bytes from p on. A load at an address that is no multiple of 4 takes several times as long
+// (16 rows of 4096 to 4096 channels at odd strides 11.9 us, at strides of 4 7.0), so with `odd` (the
+// same in the wave) they come from the whole words that they lie in, shifted into place.
+__device__ __forceinline__ v4i load16_at(const int8_t *p, bool odd) {
+    v4i v;
+    if (!odd) {
+        __builtin_memcpy(&v, p, 16);
+        return v;
+    }
+    const uint32_t back = (uint32_t)(uintptr_t)p & 3;
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(p - back), *last = w + (back ? 4 : 3);
+    __builtin_memcpy(&v, w, 16);
+    const uint32_t e = *last;
+    v4i o;
+    o[0] = (int)__builtin_amdgcn_alignbyte((uint32_t)v[1], (uint32_t)v[0], back);
+    o[1] = (int)__builtin_amdgcn_alignbyte((uint32_t)v[2], (uint32_t)v[1], back);
+    o[2] = (int)__builtin_amdgcn_alignbyte((uint32_t)v[3], (uint32_t)v[2], back);
+    o[3] = (int)__builtin_amdgcn_alignbyte(e, (uint32_t)v[3], back);
+    return o;
+}
+
+// load16 where the row's end lies at p + ok, 16 bytes or more behind its start; ok may be
+// below 0. One load and no condition: behind the end the row's last 16 bytes, moved down.
+__device__ __forceinline__ v4i load16_end(const int8_t *p, int ok) {
+    const int gone = ok >= 16 ? 0 : 16 - ok;   // bytes
+    unsigned long long h[2];
+    __builtin_memcpy(h, p - gone, 16);
+    const uint32_t bits = 8 * (gone & 7);
+    if (gone & 7) {
+        h[0] = h[0] >> bits | h[1] << (64 - bits);
+        h[1] >>= bits;
+    }
+    unsigned long long lo = gone >= 16 ? 0 : gone >= 8 ? h[1] : h[0], hi = gone >= 8 ? 0 : h[1];
+    v4i v;
+    v[0] = (int)lo;
+    v[1] = (int)(lo >> 32);
+    v[2] = (int)hi;
+    v[3] = (int)(hi >> 32);
+    return v;
+}
+
 __device__ __forceinline__ float scaled(int acc, float xs, float ws, float b) { return (float)acc * xs * ws + b; }
 __device__ __forceinline__ float relu(float y) { return y < 0.0f ? 0.0f : y; }   // NaN stays
 __device__ __forceinline__ float sigmoid(float y) {

@@ -350,6 +350,22 @@ def test_linear_floats_few_many_channels(head):
     check_linear(head, rows_of(g, 3, 300, 1, torch.float16), None, w, ws, bias, "none", torch.float32)
 
 
+@pytest.mark.parametrize("xt", [*FLOATS, "i8"])
+@pytest.mark.parametrize("rows,k,n", [(9001, 70, 1), (9001, 130, 17), (20005, 300, 32), (140000, 65, 16), (50, 3008, 5),
+                                      (50, 3009, 5), (333, 1000, 31), (17, 20000, 9), (40, 7000, 32), (33, 13000, 16),
+                                      (70003, 129, 33), (8200, 520, 12)])
+def test_linear_few_channels(head, xt, rows, k, n):
+    """Many rows to few channels, at strides that are multiples of 16 and odd ones."""
+    g = gen_of("fc", rows, k, n)
+    for pad in (-k % 16, (-k % 4) + 1):
+        w, ws, bias = layer_of(g, n, k, pad, True)
+        if xt == "i8":
+            x, xs = codes_of(g, rows, k, pad), (0.005 + 0.01 * torch.rand(rows, generator=g)).cuda()
+        else:
+            x, xs = rows_of(g, rows, k, pad, FLOATS[xt]), None
+        check_linear(head, x, xs, w, ws, bias, "none", torch.float32)
+
+
 def test_linear_far_rows(head):
     """x, weights and y beyond 2^31 elements from their first."""
     g = gen_of("far")

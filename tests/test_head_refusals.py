@@ -63,16 +63,16 @@ def lin(fake, native, work=0, work_bytes=0, **over):
     (dict(ldx=31), "apart"), (dict(ldw=31), "apart"), (dict(ldy=15), "apart"), (dict(w=None), "null"),
     (dict(ws=None), "null"), (dict(x=None), "null"), (dict(xs=None), "null"), (dict(y=None), "null"),
     (dict(bias=P + 2), "misaligned"), (dict(y=P + 2), "misaligned"), (dict(yt=1, y=P + 1), "misaligned"),
-    (dict(xt=0), "x scales given"), (dict(xt=2, xs=None, rows=200, k=500, ldx=500, ldw=500), "workspace"), (dict(rows=1 << 41), "range")])
+    (dict(xt=0), "x scales given"), (dict(xt=2, xs=None, rows=200, n=500, ldy=500, k=500, ldx=500, ldw=500), "workspace"), (dict(rows=1 << 41), "range")])
 def test_linear_refusals(fake, native, over, word):
     refused(fake, lin(fake, native, **over), word)
 
 
 def test_linear_workspace(fake, native):
-    layer = native.q8_linear(P, P, None, 100, 16)
+    layer = native.q8_linear(P, P, None, 100, 160)
     need = native.linear_q8_work(layer, native.DTYPE_F32, 1000)
     assert need >= 1000 * 104
-    over = dict(xt=0, xs=None, rows=1000, k=100, ldw=100, ldx=100)
+    over = dict(xt=0, xs=None, rows=1000, k=100, n=160, ldy=160, ldw=100, ldx=100)
     refused(fake, lin(fake, native, P, need - 1, **over), "workspace")
     refused(fake, lin(fake, native, P + 8, need, **over), "workspace")
     refused(fake, lin(fake, native, None, need, **over), "workspace")
