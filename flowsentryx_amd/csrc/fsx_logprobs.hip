@@ -17,6 +17,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct Larger { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
 struct LargerFloat { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct LargerWord { __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return max(a, b); } };
+struct PlusWord { __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return a + b; } };
 struct Plus { __device__ float operator()(float a, float b) const { return a + b; } };
 
 // An alternative: its value as an ordered word above its class, so that the largest word is
@@ -118,16 +120,34 @@ __device__ void finish_row(const LogprobArgs &a, uint64_t r, const Sums &q, Alt 
 
 // ---------------------------------------------------------------- short rows: G lanes a row
 
+// A wave's RW rows: up to KEEP alternatives of each in falling order, and for RANK their words.
+enum { kKeep, kRank, kChoose };   // how a row's alternatives are put in order
+template <int RW, int KEEP, int PITCH> struct ShortRows {
+    Alt alts[RW * KEEP];
+    uint32_t words[PITCH ? RW * PITCH : 4];
+    float2 end[RW];    // m, and log S (a bad row: NaN)
+    uint32_t found[RW];
+};
+// What the wave's lanes have written to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Up to 64 N classes: a lane holds N neighbouring logits of its row, G lanes (a power of two)
-// a row, so the row is read once and its maximum is known before the sums. An alternative is
-// the group's largest word; its lane clears it and the next round finds the next. The lanes
-// keep the results of G rounds and store them side by side. WHOLE: the classes are a multiple
-// of N, so a lane has all of its logits or none; the next rows are then under way while a
-// block works on the ones before.
-template <int DT, int N, int G, bool WHOLE>
-__global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a) {
+// a row, so the row is read once and its maximum is known before the sums. A wave's alternatives
+// are ordered in LDS and then stored side by side, all its rows' at once. Their order: RANK counts
+// for each logit the ones before it, against the row's words from LDS; else the group's largest
+// word is the next one, and the first lane that holds it clears it. WHOLE: the classes are a
+// multiple of N, so a lane has all of its logits or none; the next rows are then under way while
+// a block works on the ones before.
+template <int DT, int N, int G, bool WHOLE, int ORDER>
+__global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t top_inv) {
     using T = typename Elem<DT>::T;
-    constexpr uint32_t PER = 256 / G;
+    constexpr uint32_t PER = 256 / G, RW = 64 / G, KEEP = G * N < 64 ? G * N : 64, PITCH = G * N + 4;
+    __shared__ __attribute__((aligned(16))) ShortRows<RW, KEEP, (ORDER == kRank && G > 1 ? PITCH : 0)> s_rows[4];
+    auto &sh = s_rows[threadIdx.x >> 6];
     const uint32_t g = threadIdx.x % G, c0 = g * N;
     const uint64_t step = (uint64_t)gridDim.x * PER;
     uint64_t r = (uint64_t)blockIdx.x * PER + threadIdx.x / G;
@@ -175,45 +195,164 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a) {
         uint32_t w[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = x[i] > -INFINITY ? ord_of(x[i]) : 0u;
-        Alt mine = 0;
-        uint64_t to = r * a.top + g;
-        for (uint32_t k = 0;; ++k) {
-            uint32_t b = w[0], c = c0;
+        if constexpr (ORDER == kKeep) {
+            Alt mine = 0;
+            uint64_t to = r * a.top + g;
+            for (uint32_t k = 0;; ++k) {
+                uint32_t b = w[0], c = c0;
 #pragma unroll
-            for (int i = 1; i < N; ++i)
-                if (w[i] > b) { b = w[i]; c = c0 + i; }
-            const Alt own = b ? (Alt)b << 32 | (uint32_t)~c : 0;
-            const Alt best = group_all<G>(own, Larger());
-            const uint32_t place = k % G;
-            if (place == g) mine = best;
-            const bool last = k + 1 == a.top;
-            if (last || place == G - 1) {
-                if (g <= place && live) {
-                    a.top_id[to] = end.id(mine);
-                    a.top_lp[to] = end.id_log_p(mine);
+                for (int i = 1; i < N; ++i)
+                    if (w[i] > b) { b = w[i]; c = c0 + i; }
+                const Alt own = b ? (Alt)b << 32 | (uint32_t)~c : 0;
+                const Alt best = group_all<G>(own, Larger());
+                const uint32_t place = k % G;
+                if (place == g) mine = best;
+                const bool last = k + 1 == a.top;
+                if (last || place == G - 1) {
+                    if (g <= place && live) {
+                        a.top_id[to] = end.id(mine);
+                        a.top_lp[to] = end.id_log_p(mine);
+                    }
+                    if (last) break;
+                    to += G;
                 }
-                if (last) break;
-                to += G;
-            }
-            const uint32_t gone = (uint32_t)~(uint32_t)best;   // (in its own lane one of c0 .. c0 + N - 1)
+                const uint32_t gone = (uint32_t)~(uint32_t)best;   // (in its own lane one of c0 .. c0 + N - 1)
 #pragma unroll
-            for (int i = 0; i < N; ++i) w[i] = gone == c0 + i ? 0 : w[i];
+                for (int i = 0; i < N; ++i) w[i] = gone == c0 + i ? 0 : w[i];
+            }
+            continue;
         }
+        const uint32_t lane = lane_now(), row = lane / G;
+        Alt *to = sh.alts + row * KEEP;
+        if (g == 0) sh.end[row] = {end.m, end.bad ? NAN : end.empty ? 0.0f : end.ls};
+        uint32_t found = 0;   // alternatives of the row
+        if constexpr (ORDER == kRank) {
+            uint32_t rank[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) rank[i] = 0;
+            if constexpr (G == 1) {
+#pragma unroll
+                for (int j = 1; j < N; ++j)
+#pragma unroll
+                    for (int i = 0; i < j; ++i) {
+                        const bool before = w[i] >= w[j];
+                        rank[j] += before ? 1 : 0;
+                        rank[i] += before ? 0 : 1;
+                    }
+            } else {
+                uint32_t *words = sh.words + row * PITCH;
+#pragma unroll
+                for (int i = 0; i < N; i += 4)
+                    *reinterpret_cast<uint4 *>(words + c0 + i) = uint4{w[i], w[i + 1], w[i + 2], w[i + 3]};
+                wave_sync();
+#pragma unroll 1
+                for (uint32_t j = 0; j < a.v; j += 4) {
+                    const uint4 o4 = *reinterpret_cast<const uint4 *>(words + j);
+                    const uint32_t o[4] = {o4.x, o4.y, o4.z, o4.w}, ties = j < c0 ? 1 : 0;   // (equal: the lower class)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int i = 0; i < N; ++i) rank[i] += o[e] + ties > w[i] ? 1 : 0;
+                }
+#pragma unroll
+                for (int j = 1; j < N; ++j)
+#pragma unroll
+                    for (int i = 0; i < j; ++i) rank[j] += w[i] == w[j] ? 1 : 0;
+                wave_sync();   // (the next rows' words come to the same place)
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                found += w[i] ? 1 : 0;
+                if (w[i] && rank[i] < a.top) to[rank[i]] = (Alt)w[i] << 32 | (uint32_t)~(c0 + i);
+            }
+            found = group_all<G>(found, PlusWord());
+        } else {
+            const uint32_t most = a.top < a.v ? a.top : a.v;
+            const uint64_t before = ((1ull << lane) - 1) & ~((1ull << (lane & ~(uint32_t)(G - 1))) - 1);   // of the group
+#pragma unroll 1
+            for (uint32_t k = 0; k < most; ++k) {
+                uint32_t b = w[0];
+#pragma unroll
+                for (int i = 1; i < N; ++i) b = max(b, w[i]);
+                const uint32_t best = group_all<G>(b, LargerWord());
+                if (!__ballot(best != 0)) break;
+                found += best ? 1 : 0;
+                const uint64_t holders = __ballot(b == best);
+                if (b == best && best && !(holders & before)) {
+                    uint32_t c = c0;
+                    bool gone = false;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const bool it = !gone && w[i] == best;
+                        c = it ? c0 + i : c;
+                        w[i] = it ? 0 : w[i];
+                        gone = gone || it;
+                    }
+                    to[k] = (Alt)best << 32 | (uint32_t)~c;
+                }
+            }
+        }
+        if (g == 0) sh.found[row] = found;
+        wave_sync();
+        const uint64_t r0 = b0 + (threadIdx.x >> 6) * RW;
+        const uint32_t rows = r0 >= a.rows ? 0 : a.rows - r0 < RW ? (uint32_t)(a.rows - r0) : RW;
+#pragma unroll 1
+        for (uint32_t i = lane; i < rows * a.top; i += 64) {
+            const uint32_t q = i * top_inv >> 18, k = i - q * a.top;   // i / top: i < 2^12
+            const float2 e = sh.end[q];
+            const Alt alt = k < sh.found[q] ? sh.alts[q * KEEP + k] : 0;
+            const bool none = alt == 0, bad = e.y != e.y;
+            a.top_id[r0 * a.top + i] = bad || none ? -1 : (int32_t)~(uint32_t)alt;
+            a.top_lp[r0 * a.top + i] = bad ? NAN : none ? -INFINITY : (value_of((uint32_t)(alt >> 32)) - e.x) - e.y;
+        }
+        wave_sync();
     }
 }
 
 template <int DT, int N, int G> static bool logprobs_short(const LogprobArgs &a, hipStream_t st) {
     const uint64_t blocks = (a.rows + 256 / G - 1) / (256 / G);
     const uint32_t grid = (uint32_t)std::min<uint64_t>(blocks, 256 * 8);   // (the blocks that fit at once)
-    if (a.v % N == 0) k_logprobs_short<DT, N, G, true><<<grid, 256, 0, st>>>(a);
-    else k_logprobs_short<DT, N, G, false><<<grid, 256, 0, st>>>(a);
+    const uint32_t top_inv = a.top ? ((1u << 18) + a.top - 1) / a.top : 0;
+    // A few alternatives: kept in registers and stored as they come (us of 2^22 rows of 16 f32 logits,
+    // 1 / 3 / 5 alternatives: 84 / 110 / 145, by way of LDS 93 / 114 / 147; 200000 rows of 33, 3 / 5 / 8: 26 /
+    // 34 / 45 and 26 / 31 / 38). Counting costs what the row is long, choosing what is asked for: about
+    // v (2 N + 2) and 3 / 5 top (4 N + 3 log2 G + 14) instructions a lane (33 classes: counting 51 us, choosing
+    // 18 + 2.4 top; 2^20 rows of 7 f16 logits, 28 asked for: 64 us, where one by one took 376).
+    constexpr uint32_t log_g = G > 32 ? 6 : G > 16 ? 5 : G > 8 ? 4 : G > 4 ? 3 : G > 2 ? 2 : G > 1 ? 1 : 0;
+    const uint32_t rank_cost = G == 1 ? 2 * N * N : a.v * (2 * N + 2),
+                   rounds_cost = std::min(a.top, a.v) * (4 * N + 3 * log_g + 14);
+    auto go = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(a, top_inv); };
+    if (a.top <= 3) {
+        if (a.v % N == 0) go(k_logprobs_short<DT, N, G, true, kKeep>);
+        else go(k_logprobs_short<DT, N, G, false, kKeep>);
+        return true;
+    }
+    if constexpr (G * N <= 512) {
+        if (5 * rank_cost < 3 * rounds_cost) {
+            if (a.v % N == 0) go(k_logprobs_short<DT, N, G, true, kRank>);
+            else go(k_logprobs_short<DT, N, G, false, kRank>);
+            return true;
+        }
+    }
+    if (a.v % N == 0) go(k_logprobs_short<DT, N, G, true, kChoose>);
+    else go(k_logprobs_short<DT, N, G, false, kChoose>);
     return true;
 }
 // 16 bytes a lane as far as 64 lanes reach; then 16 logits a lane
 constexpr uint32_t kShort = 64 * 16;
+constexpr uint64_t kManyRows = 1024;   // for long rows: blocks of four waves from here on
+constexpr uint32_t kFewTop = 32;       // up to here a bound from 64 words does; beyond, from 256
+// Of the longer of these rows, more than a few alternatives are sooner found by a block that bounds
+// them, if it has lanes enough for the bound (us with 20 of 1004 logits, 200 / 700 / 3000 rows: 15.6 /
+// 14.6 / 23.3 here, 5.7 / 9.9 / 14.4 there; of 500: 10.0 / 9.9 / 12.5 and 5.7 / 9.8 / 12.8; 64 of 500: 24.5 and 45.7).
+static bool is_short(uint64_t rows, uint32_t v, uint32_t top) {
+    if (v > kShort) return false;
+    if (top <= 5 || v < (top > kFewTop ? 15 : 10) * top) return true;
+    return rows <= 256 ? v <= 128 : v <= 512 || (rows >= kManyRows && top > kFewTop);
+}
 template <int DT> static bool logprobs_short(const LogprobArgs &a, hipStream_t st) {
     constexpr int N = DT == FSX_DTYPE_F32 ? 4 : 8;
-    if (a.v > kShort) return false;
+    if (!is_short(a.rows, a.v, a.top)) return false;
     if (a.v <= 1 * N) return logprobs_short<DT, N, 1>(a, st);
     if (a.v <= 2 * N) return logprobs_short<DT, N, 2>(a, st);
     if (a.v <= 4 * N) return logprobs_short<DT, N, 4>(a, st);
@@ -251,7 +390,6 @@ template <int WORDS> __device__ uint32_t nth_largest(const uint32_t (&w)[WORDS],
 // from counting for each how many are larger (their words all differ), so no list is kept
 // sorted and no lane waits for another.
 constexpr uint32_t kPool = 128;   // a wave's candidates: 64 alternatives and one of every lane
-constexpr uint32_t kFewTop = 32;  // up to here a bound from 64 words does; beyond, from 256
 template <int W> struct Shared {
     Alt pool[W][kPool];
     Alt all[W * kPool];
@@ -552,7 +690,6 @@ __global__ __launch_bounds__(256) void k_logprobs_join(LogprobArgs a, uint32_t p
 
 // Many rows: a block of four waves each. Fewer: of sixteen, each with less to do, and with
 // fewer rows than half the CUs a row in parts, a round for every block at least.
-static constexpr uint64_t kManyRows = 1024;
 static constexpr int kFewW = 16, kFewH = 1;
 static uint32_t long_parts(uint64_t rows, uint32_t v) {
     if (v <= kShort || rows >= kManyRows) return 1;

@@ -514,6 +514,28 @@ def test_logprobs_orders(head, rows, classes, top):
     check_logprobs(head, x.cuda(), top=top)
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows", [1, 70, 300, 1100])
+@pytest.mark.parametrize("classes,top", [(3, 4), (4, 64), (7, 28), (8, 4), (9, 9), (16, 5), (20, 22), (25, 4), (33, 33),
+                                         (64, 4), (84, 19), (129, 6), (129, 12), (130, 64), (256, 25), (278, 30), (513, 6),
+                                         (520, 40), (700, 46), (1000, 64), (1004, 20), (1023, 7)])
+def test_logprobs_short_orders(head, dtype, rows, classes, top):
+    """Each way that the alternatives of short rows are put in order: ties, masked and empty rows,
+    more asked for than there are."""
+    g = gen_of("so", rows, classes, top)
+    x = 3 * torch.randn(rows, classes + 1, generator=g)
+    x[::3] = torch.randint(-2, 3, (len(x[::3]), classes + 1), generator=g).float()
+    x[1::4][torch.rand(len(x[1::4]), classes + 1, generator=g) < 0.9] = NEG
+    x[-1] = NEG
+    if rows > 40:
+        x[20], x[21] = 1.0, NEG
+        x[21, classes - 1] = 0.5
+        x[22, classes // 2] = float("nan")
+        x[23, 0] = float("inf")
+        x[24] = torch.arange(classes + 1) / classes
+    check_logprobs(head, x.to(FLOATS[dtype]).cuda()[:, :classes], top=top)
+
+
 def test_logprobs_parts(head):
     """Each output by itself, and none of them but the alternatives."""
     for classes in (16, 300, 5000, 70000):
