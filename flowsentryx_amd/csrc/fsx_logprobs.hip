@@ -338,17 +338,16 @@ template <int DT, int N, int G> static bool logprobs_short(const LogprobArgs &a,
     else go(k_logprobs_short<DT, N, G, false, kChoose>);
     return true;
 }
-// 16 bytes a lane as far as 64 lanes reach; then 16 logits a lane
-constexpr uint32_t kShort = 64 * 16;
+// 16 bytes a lane as far as 64 lanes reach (3000 rows of 600 logits and up are faster in blocks: with 3 /
+// 20 alternatives 10.4 / 20 us at 16 logits a lane, 9.9 / 11.2 there; of 1004: 13.3 / 23 and 9.6 / 11.2)
+constexpr uint32_t kShort = 64 * 8;
 constexpr uint64_t kManyRows = 1024;   // for long rows: blocks of four waves from here on
 constexpr uint32_t kFewTop = 32;       // up to here a bound from 64 words does; beyond, from 256
 // Of the longer of these rows, more than a few alternatives are sooner found by a block that bounds
-// them, if it has lanes enough for the bound (us with 20 of 1004 logits, 200 / 700 / 3000 rows: 15.6 /
-// 14.6 / 23.3 here, 5.7 / 9.9 / 14.4 there; of 500: 10.0 / 9.9 / 12.5 and 5.7 / 9.8 / 12.8; 64 of 500: 24.5 and 45.7).
+// them, if it has lanes enough for the bound (us with 5 / 20 / 64 of 500 logits, 1500 rows: 5.6 / 10.5 /
+// 24.9 here, 6.6 / 7.1 / 47.6 there; 20000 rows: 23 / 48 / 124 and 43 / 48 / 439).
 static bool is_short(uint64_t rows, uint32_t v, uint32_t top) {
-    if (v > kShort) return false;
-    if (top <= 5 || v < (top > kFewTop ? 15 : 10) * top) return true;
-    return rows <= 256 ? v <= 128 : v <= 512 || (rows >= kManyRows && top > kFewTop);
+    return v <= kShort && (v <= 128 || top <= (rows <= 2048 ? 5 : 20) || v < (top > kFewTop ? 15 : 10) * top);
 }
 template <int DT> static bool logprobs_short(const LogprobArgs &a, hipStream_t st) {
     constexpr int N = DT == FSX_DTYPE_F32 ? 4 : 8;
@@ -360,8 +359,7 @@ template <int DT> static bool logprobs_short(const LogprobArgs &a, hipStream_t s
     if (a.v <= 16 * N) return logprobs_short<DT, N, 16>(a, st);
     if (a.v <= 32 * N) return logprobs_short<DT, N, 32>(a, st);
     if (a.v <= 64 * N) return logprobs_short<DT, N, 64>(a, st);
-    if constexpr (DT == FSX_DTYPE_F32) if (a.v <= 32 * 16) return logprobs_short<DT, 16, 32>(a, st);
-    return logprobs_short<DT, 16, 64>(a, st);
+    return logprobs_short<DT, 8, 64>(a, st);   // (f32: 32 bytes a lane)
 }
 
 // ---------------------------------------------------------------- long rows: blocks of W waves
@@ -515,7 +513,7 @@ __device__ __forceinline__ void block_pass(Shared<W> &sh, const typename Elem<DT
             __builtin_memcpy(raw[h], x + (c < end ? c : end), sizeof(raw[h]));
         }
     };
-    constexpr bool AHEAD = H == 1;   // (with more reads a lane the registers go to more waves)
+    constexpr bool AHEAD = H == 1 && W == 16;   // (else a row is one round or few, or the registers go to more waves)
     if (AHEAD) read((part * W + wave) * kPiece + lane * kLV);
 #pragma unroll 1
     for (uint32_t block_at = part * W * kPiece; block_at < v; block_at += step, ++round) {   // (< 2^32)
@@ -701,7 +699,13 @@ template <int DT, bool TOP>
 static void logprobs(const LogprobArgs &a, hipStream_t st) {
     const uint32_t parts = long_parts(a.rows, a.v);
     const dim3 grid(parts, (uint32_t)std::min<uint64_t>(a.rows, 65535));
-    if (a.rows >= kManyRows) k_logprobs_long<DT, 4, 4, TOP><<<grid, 64 * 4, 0, st>>>(a, 1);
+    // Pieces as large as all waves of a block have some: 20000 rows of 2048 with 1 / 20 / 64 alternatives 41 /
+    // 52 / 75 us with pieces of 512, 47 / 68 / 950 with 2048; 9183 rows of 3199, 20 alternatives, pieces of
+    // 512 / 1024 / 2048: 38 / 32 / 39; 10000 of 5000: 50 / 50 / 45. 700 rows of 2048: 5.5 - 8.2 us, with sixteen waves
+    // a row 8.6 - 12.8.
+    if (a.v <= 2048) k_logprobs_long<DT, 4, 1, TOP><<<grid, 64 * 4, 0, st>>>(a, 1);
+    else if (a.rows >= kManyRows && a.v <= 4096) k_logprobs_long<DT, 4, 2, TOP><<<grid, 64 * 4, 0, st>>>(a, 1);
+    else if (a.rows >= kManyRows) k_logprobs_long<DT, 4, 4, TOP><<<grid, 64 * 4, 0, st>>>(a, 1);
     else k_logprobs_long<DT, kFewW, kFewH, TOP><<<grid, 64 * kFewW, 0, st>>>(a, parts);
     if (parts > 1) k_logprobs_join<DT, TOP><<<(uint32_t)std::min<uint64_t>(a.rows, 1u << 16), 256, 0, st>>>(a, parts);
 }
