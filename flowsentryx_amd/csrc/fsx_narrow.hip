@@ -30,26 +30,33 @@ __global__ __launch_bounds__(256, TN == 1 && !PART && XT != FSX_DTYPE_I8 ? 6 : 3
         ch[i].load(a, n0 + 16 * i + 4 * lq);
     }
     const uint64_t step = (uint64_t)gridDim.x * 4 * 16 * GROUPS;
-    for (uint64_t r0 = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 * GROUPS; r0 < a.rows; r0 += step) {
-        const uint64_t r = r0 + 16 * my_group + lr, rr = r < a.rows ? r : a.rows - 1;
-        const int64_t ok = (int64_t)a.k - 16 * chunk;
-        v4i x;
-        float xs;
+    uint64_t r0 = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 * GROUPS;
+    const int64_t ok = (int64_t)a.k - 16 * chunk;
+    // the next rows of x are under way while a wave works on the ones before
+    RawChunk<XT == FSX_DTYPE_I8 ? FSX_DTYPE_F32 : XT> raw;
+    v4i next_x = {0, 0, 0, 0};
+    float next_scale = 0.0f;
+    auto fetch = [&](uint64_t at) {
+        const uint64_t r = at + 16 * my_group + lr, rr = r < a.rows ? r : a.rows - 1;
         if constexpr (XT == FSX_DTYPE_I8) {
-            x = load16(static_cast<const int8_t *>(a.x) + rr * a.ldx + 16 * chunk, ok);
-            xs = a.x_scale[rr];
-        } else {
-            RawChunk<XT> raw;
-            uint32_t m = 0;
-            if (ok > 0) {
-                raw.template load<PART>(static_cast<const typename Elem<XT>::T *>(a.x) + rr * a.ldx + 16 * chunk, ok);
-                m = raw.mag();
-            }
+            next_x = load16(static_cast<const int8_t *>(a.x) + rr * a.ldx + 16 * chunk, ok);
+            next_scale = a.x_scale[rr];
+        } else if (ok > 0) {
+            raw.template load<PART>(static_cast<const typename Elem<XT>::T *>(a.x) + rr * a.ldx + 16 * chunk, ok);
+        }
+    };
+    fetch(r0);
+    for (; r0 < a.rows; r0 += step) {
+        v4i x = next_x;
+        float xs = next_scale;
+        if constexpr (XT != FSX_DTYPE_I8) {
+            uint32_t m = ok > 0 ? raw.mag() : 0;
             if (CH > 1) m = max(m, xor_lane<16>(m));
             if (CH > 2) m = max(m, xor_lane<32>(m));
             xs = row_scale(mag_value<XT>(m));
             x = ok > 0 && xs == xs ? raw.codes(1.0f / xs, xs, a.k) : v4i{0, 0, 0, 0};
         }
+        if (r0 + step < a.rows) fetch(r0 + step);
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
             v4i xg, acc[TN];
@@ -75,9 +82,12 @@ __global__ __launch_bounds__(256, TN == 1 && !PART && XT != FSX_DTYPE_I8 ? 6 : 3
 }
 
 template <int XT, int CH, int TN, int YT> static void linear_narrow(const LinearArgs &a, hipStream_t st) {
+    // (more blocks than fit at once only while a block's start, its weights, is short: 2^20 rows of 63 to 64
+    // channels 124 us with 4096 blocks, 114 with 2048; 2^22 rows of 8 to 16 118 and 121)
+    constexpr uint32_t BLOCKS = TN == 1 ? 4096 : 2048;
     const uint64_t waves = (a.rows + 16 * (4 / CH) - 1) / (16 * (4 / CH));
     const uint32_t gy = (a.n + 16 * TN - 1) / (16 * TN);
-    const dim3 grid((uint32_t)std::min<uint64_t>((waves + 3) / 4, std::max<uint32_t>(1, 4096 / gy)), gy);
+    const dim3 grid((uint32_t)std::min<uint64_t>((waves + 3) / 4, std::max<uint32_t>(1, BLOCKS / gy)), gy);
     if (XT == FSX_DTYPE_I8 || a.k % 8 == 0) k_linear_narrow<XT, CH, TN, YT, false><<<grid, 256, 0, st>>>(a);
     else k_linear_narrow<XT, CH, TN, YT, XT != FSX_DTYPE_I8><<<grid, 256, 0, st>>>(a);
 }
