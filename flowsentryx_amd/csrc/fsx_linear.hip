@@ -656,12 +656,17 @@ struct LinearPlan {
     }
 };
 
-// Large tiles read least for each product; with fewer of them than the CUs, smaller ones. us at
-// 512 / 1024 / 2048 / 4096 rows of 4096 to 4096 channels:
+// Large tiles read least for each product; with fewer of them than the CUs, smaller ones, of which
+// several share a CU: then also some load or store while others multiply. us at 512 / 1024 / 2048 /
+// 4096 rows of 4096 to 4096 channels:
 //                      256 x 256     54    55    57    70    (8192 cubed: 507)
 //   128 x 128, two buffers           26    28    37    71-77 (572)
 //   128 x 128, four buffers          23    25    55    95    (one block a CU)
 //    64 x 64                         16    33    64   119    (909)
+// Over a short k what a tile loads and stores first and last counts, and 256 x 256 with one block a CU
+// has nothing beside it: 8192 rows of 256 / 2048 to 8192 channels 119 / 215 us, 128 x 128 81 / 200. Up
+// to 64 channels larger tiles multiply zeros: 100000 rows of 256 to 64 24 us, 128 x 128 14.0, 64 x 64
+// 14.2, with half the k at a time 11.4.
 // Eight waves a block in each: four waves of twice the size were 12 - 60 % slower, since a wave
 // by itself issues an instruction in 8 cycles.
 static void linear_tiles(const LinearArgs &a, int yt, const LinearPlan &ks, void *sums_at, hipStream_t st) {
@@ -677,7 +682,8 @@ static void linear_tiles(const LinearArgs &a, int yt, const LinearPlan &ks, void
     }
     auto tiles = [&](uint64_t size) { return (a.n + size - 1) / size * ((a.rows + size - 1) / size); };
     if (dma_can(a.x, a.ldx) && dma_can(a.w, a.ldw)) {
-        if (tiles(256) >= 256) linear_tile<16, 256, 256, 128, 64, 128, 2, true>(a, yt, st);
+        if (a.n <= 64 && tiles(64) >= 256) linear_tile<16, 64, 64, 32, 16, 128, 2, true>(a, yt, st);
+        else if (a.k > 2048 && tiles(256) >= 256) linear_tile<16, 256, 256, 128, 64, 128, 2, true>(a, yt, st);
         else if (tiles(128) >= 320) linear_tile<16, 128, 128, 64, 32, 128, 2, true>(a, yt, st);
         else if (tiles(128) >= 192) linear_tile<16, 128, 128, 64, 32, 128, 4, true>(a, yt, st);
         else linear_tile<16, 64, 64, 32, 16, 256, 2, true>(a, yt, st);
