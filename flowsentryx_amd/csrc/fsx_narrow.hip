@@ -25,8 +25,9 @@ __global__ __launch_bounds__(256, TN == 1 && !PART && XT != FSX_DTYPE_I8 ? 6 : 3
     Channels ch[TN];
 #pragma unroll
     for (int i = 0; i < TN; ++i) {
-        const uint64_t c = n0 + 16 * i + lr;
-        w[i] = load16(a.w + (c < a.n ? c : a.n - 1) * a.ldw + 16 * chunk, (int64_t)a.k - 16 * chunk);
+        const uint64_t c = n0 + 16 * i + lr, cc = c < a.n ? c : a.n - 1;
+        w[i] = load16_there(a.w + cc * a.ldw + 16 * chunk, (int64_t)a.k - 16 * chunk,
+                            (int64_t)((a.n - 1 - cc) * a.ldw) + (int64_t)a.k - 16 * chunk);
         ch[i].load(a, n0 + 16 * i + 4 * lq);
     }
     const uint64_t step = (uint64_t)gridDim.x * 4 * 16 * GROUPS;
@@ -38,11 +39,12 @@ __global__ __launch_bounds__(256, TN == 1 && !PART && XT != FSX_DTYPE_I8 ? 6 : 3
     float next_scale = 0.0f;
     auto fetch = [&](uint64_t at) {
         const uint64_t r = at + 16 * my_group + lr, rr = r < a.rows ? r : a.rows - 1;
+        const int64_t there = (int64_t)((a.rows - 1 - rr) * a.ldx) + ok;   // from here to the last row's end
         if constexpr (XT == FSX_DTYPE_I8) {
-            next_x = load16(static_cast<const int8_t *>(a.x) + rr * a.ldx + 16 * chunk, ok);
+            next_x = load16_there(static_cast<const int8_t *>(a.x) + rr * a.ldx + 16 * chunk, ok, there);
             next_scale = a.x_scale[rr];
         } else if (ok > 0) {
-            raw.template load<PART>(static_cast<const typename Elem<XT>::T *>(a.x) + rr * a.ldx + 16 * chunk, ok);
+            raw.template load<PART>(static_cast<const typename Elem<XT>::T *>(a.x) + rr * a.ldx + 16 * chunk, ok, there);
         }
     };
     fetch(r0);
@@ -97,7 +99,8 @@ template <int XT, int CH, int TN> static void linear_narrow(const LinearArgs &a,
     else linear_narrow<XT, CH, TN, FSX_DTYPE_BF16>(a, st);
 }
 template <int XT, int CH> static void linear_narrow(const LinearArgs &a, int yt, hipStream_t st) {
-    if (a.n <= 16) linear_narrow<XT, CH, 1>(a, yt, st);
+    // (64 channels a wave, or 16 where that leaves SIMDs without one)
+    if (a.n <= 16 || (a.rows * CH / 64 + 1) * (a.n / 64 + 1) < 2048) linear_narrow<XT, CH, 1>(a, yt, st);
     else linear_narrow<XT, CH, 4>(a, yt, st);
 }
 template <int XT> static void linear_narrow(const LinearArgs &a, int yt, hipStream_t st) {

@@ -72,8 +72,8 @@ template <int DT> struct RawChunk {   // kQV values as they lie in memory
     using T = typename Elem<DT>::T;
     static constexpr int WORDS = kQV * sizeof(T) / 4;
     uint32_t w[WORDS];
-    // ok > 0 values exist, behind them: 0 (PART false: a whole number of eights)
-    template <bool PART = true> __device__ __forceinline__ void load(const T *p, int64_t ok) {
+    // ok > 0 values count, behind them: 0 (PART false: a whole number of eights). `there` values can be read.
+    template <bool PART = true> __device__ __forceinline__ void load(const T *p, int64_t ok, int64_t there = 0) {
         if (ok >= kQV) {
             __builtin_memcpy(w, p, sizeof(w));
             return;
@@ -84,6 +84,13 @@ template <int DT> struct RawChunk {   // kQV values as they lie in memory
             const int64_t here = ok - 8 * h;
             if (here >= 8) {
                 __builtin_memcpy(half, p + 8 * h, sizeof(w) / 2);
+            } else if (PART && here > 0 && there >= 8 * h + 8) {   // (the next row's; they are read in one and cleared)
+                __builtin_memcpy(half, p + 8 * h, sizeof(w) / 2);
+#pragma unroll
+                for (int i = 0; i < WORDS / 2; ++i) {
+                    const int64_t values = here - (int64_t)(i * (4 / sizeof(T)));   // of this word on
+                    half[i] = values <= 0 ? 0 : values == 1 && sizeof(T) == 2 ? half[i] & 0xFFFFu : half[i];
+                }
             } else if (PART && here > 0) {
                 T t[8];
 #pragma unroll
@@ -151,6 +158,19 @@ __device__ __forceinline__ v4i load16(const int8_t *p, int64_t ok) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) b[i] = i < ok ? b[i] : (int8_t)0;
         __builtin_memcpy(&v, b, 16);
+    }
+    return v;
+}
+
+// load16 where `there` bytes can be read from p on (the next rows'): then in one load, and cleared.
+__device__ __forceinline__ v4i load16_there(const int8_t *p, int64_t ok, int64_t there) {
+    if (there < 16) return load16(p, ok);
+    v4i v;
+    __builtin_memcpy(&v, p, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int left = (int)ok - 4 * i;   // of this word on
+        v[i] &= left >= 4 ? -1 : left <= 0 ? 0 : (int)((1u << (8 * left)) - 1);
     }
     return v;
 }

@@ -366,6 +366,21 @@ def test_linear_few_channels(head, xt, rows, k, n):
         check_linear(head, x, xs, w, ws, bias, "none", torch.float32)
 
 
+@pytest.mark.parametrize("xt", [*FLOATS, "i8"])
+@pytest.mark.parametrize("rows,k,n", [(140001, 5, 20), (70001, 16, 100), (33000, 17, 130), (40000, 31, 65), (9000, 40, 700),
+                                      (3000, 64, 3000), (2, 7, 300), (70000, 7, 12)])
+def test_linear_short_rows(head, xt, rows, k, n):
+    """Rows of up to 64 values to few channels and many, beside each other and apart."""
+    g = gen_of("short", rows, k, n)
+    for pad in (0, 3):
+        w, ws, bias = layer_of(g, n, k, pad, True)
+        if xt == "i8":
+            x, xs = codes_of(g, rows, k, pad), (0.005 + 0.01 * torch.rand(rows, generator=g)).cuda()
+        else:
+            x, xs = rows_of(g, rows, k, pad, FLOATS[xt]), None
+        check_linear(head, x, xs, w, ws, bias, "relu", torch.bfloat16)
+
+
 def test_linear_far_rows(head):
     """x, weights and y beyond 2^31 elements from their first."""
     g = gen_of("far")
