@@ -715,10 +715,16 @@ static void slabs(const LinearArgs &a, int y_dtype, uint32_t x_size, F launch) {
     }
 }
 
-// What a call needs; without a pointer: as if those rows were at odd strides.
+// What a call needs; without a pointer: at any place of those rows (the forms differ, and none needs
+// the most at all sizes).
 uint64_t linear_work(uint64_t rows, uint32_t k, uint32_t n, int x_dtype, const void *x, uint64_t ldx, const void *w,
                      uint64_t ldw) {
-    return LinearPlan(rows, k, n, x_dtype, x && dma_can(x, ldx), w && dma_can(w, ldw)).bytes();
+    uint64_t most = 0;
+    for (const bool x_fits : {false, true})
+        for (const bool w_fits : {false, true})
+            if ((!x || x_fits == dma_can(x, ldx)) && (!w || w_fits == dma_can(w, ldw)))
+                most = std::max(most, LinearPlan(rows, k, n, x_dtype, x_fits, w_fits).bytes());
+    return most;
 }
 
 static void pack_rows(const int8_t *p, uint64_t ld, uint64_t rows, uint32_t k, int8_t *to, hipStream_t st) {

@@ -253,7 +253,7 @@ TILES = [(4097, 130, 4000, 14, 14), (4097, 70, 4000, 10, 10), (2300, 100, 2305, 
          (1700, 70, 1801, 10, 10), (1700, 200, 1801, 8, 8), (1700, 390, 1801, 10, 10), (1700, 700, 1801, 4, 4),
          (300, 65, 400, 15, 15), (300, 520, 400, 8, 8), (300, 65, 400, 0, 15), (300, 777, 403, 0, 0),
          (2100, 333, 2100, 0, 0), (2100, 333, 2100, 3, 0), (2100, 333, 2100, 0, 3), (4100, 65, 4100, 1, 2),
-         (100, 5000, 200, 8, 8), (100, 5001, 200, 0, 0), (17, 2048, 100, 0, 0), (40, 2049, 7, 15, 15), (40, 2049, 7, 0, 15),
+         (100, 5000, 200, 8, 8), (100, 5001, 200, 0, 0), (17, 2048, 100, 0, 0), (4000, 2000, 320, 0, 1), (700, 2000, 2000, 0, 15), (40, 2049, 7, 15, 15), (40, 2049, 7, 0, 15),
          (33, 131071, 65, 1, 1), (20, 4096, 16390, 0, 0), (2, 16400, 100, 0, 0), (16, 9000, 2050, 8, 8),
          (17000, 130, 50, 14, 14), (17001, 300, 64, 4, 4), (4097, 2050, 4000, 14, 14), (9, 9001, 130, 0, 0), (16, 300, 9000, 4, 4), (31, 300, 8000, 4, 5)]
 

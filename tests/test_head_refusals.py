@@ -3,6 +3,7 @@ fsx_linear_q8_device, fsx_logprobs_device), their workspace sizes, and the 64-bi
 own known answers. A refused call touches nothing but the context's message, so a zeroed block
 of memory stands in for a context here."""
 import ctypes as C
+import random
 import errno
 import math
 
@@ -89,6 +90,27 @@ def test_linear_workspace_before_the_weights(fake, native):
     for rows, k, n, ld in ((5000, 512, 5000, 512), (5000, 500, 5000, 500), (100, 4096, 64, 4096), (2, 9, 5, 9)):
         sizes = [native.linear_q8_work(native.q8_linear(w, P, None, k, n, ld), native.DTYPE_I8, rows) for w in (P, P + 1, None)]
         assert sizes[2] == max(sizes), (rows, k, n, ld)
+
+
+def test_linear_takes_the_workspace_it_asks_for(fake, native):
+    """Whatever the sizes and places, a workspace of the size asked for is enough for the call (which
+    fails later here, without a GPU)."""
+    if torch.cuda.device_count():
+        pytest.skip("with a GPU the accepted calls would run, on addresses that are none")
+    rng = random.Random(5)
+    lib, ctx, _ = fake
+    size = lambda top: int(round(2 ** rng.uniform(0, top)))
+    cases = [(4000, 2000, 320, 3, 0, 1, 0)]
+    for _ in range(4000):
+        cases.append((size(20), min(131071, size(17)), size(16), rng.choice((0, 2, 3, 3)), rng.choice((0, 0, 1, 8)),
+                      rng.choice((0, 0, 1, 8)), rng.choice((0, 0, 4))))
+    for rows, k, n, xt, xpad, wpad, at in cases:
+        ldx, ldw = k + -k % 16 + xpad, k + -k % 16 + wpad
+        layer = native.q8_linear(P + at, P, None, k, n, ldw)
+        need = native.linear_q8_work(layer, xt, rows)
+        lin(fake, native, P, need, w=P + at, k=k, n=n, ldw=ldw, xt=xt, ldx=ldx, xs=P if xt == 3 else None, rows=rows,
+            x=P + at, ldy=n)
+        assert b"workspace" not in lib.fsx_last_error(ctx), (rows, k, n, xt, ldx, ldw, at, lib.fsx_last_error(ctx))
 
 
 def logp(fake, work=0, work_bytes=0, **over):
