@@ -600,8 +600,9 @@ static bool dma_can(const void *p, uint64_t ld) { return ((uintptr_t)p | ld) % 1
 // kTiles: k_linear_tile.
 //
 // Few blocks over a long k are cut into parts; the join is another launch. In tiles: 40 rows of
-// 10931 to 42 channels 14.3 us in 10 parts, 13.3 in 20. Direct: 14 rows of 11313 to 1384 channels
-// 24 -> 12.8, but one row of 4096 to 1024 channels 4.8 -> 7.1: by the bytes that a block takes.
+// 10931 to 42 channels 14.3 us in 10 parts, 13.3 in 20; through registers more tiles are cut (107
+// rows of 6581 to 6892 channels 57 -> 38) than by DMA (603 rows of 3982 to 1394 22.6 -> 25.9: not).
+// Direct: 14 rows of 11313 to 1384 channels 24 -> 12.8, but one row of 4096 to 1024 channels 4.8 -> 7.1: by the bytes that a block takes.
 // Operands that the DMA cannot bring are packed for it where the work repays the copy: 4096 rows
 // of 4096 to 4096 channels at odd strides 182 -> 78 us, 1006 rows of 8444 to 2643 channels 104 ->
 // 64, but 1000 rows of 1003 to 777 channels 8.0 -> 12.2.
@@ -652,7 +653,8 @@ struct LinearPlan {
             if (pack_w) w_bytes = n * up16(k);
         }
         const uint64_t tiles = (n + 63ull) / 64 * ((rows + 63) / 64);
-        if (tiles < 128 && k >= 2048) cut(tiles, 512, 512);
+        const bool dma = (x_fits || pack_x) && (w_fits || pack_w);
+        if (tiles < 128 ? k >= (dma ? 2048 : 1024) : !dma && tiles < 256 && k >= 4096) cut(tiles, 512, 512);
     }
 };
 
