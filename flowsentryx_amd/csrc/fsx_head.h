@@ -72,24 +72,6 @@ template <> struct Elem<FSX_DTYPE_F32> { using T = float; };
 template <> struct Elem<FSX_DTYPE_F16> { using T = _Float16; };
 template <> struct Elem<FSX_DTYPE_BF16> { using T = __bf16; };
 
-// N elements of T from p on (any alignment of p that T has: global loads need no more), of
-// which the first `ok` exist; the others are `fill`.
-template <typename T, int N>
-__device__ __forceinline__ void load_row(const T *p, int64_t ok, float fill, float (&v)[N]) {
-    T t[N];
-    if (ok >= N) {
-        __builtin_memcpy(t, p, sizeof(t));
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = (float)t[i];
-    } else {
-        // (loads without conditions, behind the end the first element again: all are under way at once)
-        if (ok > 0)
-#pragma unroll
-            for (int i = 0; i < N; ++i) t[i] = p[i < ok ? i : 0];
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = i < ok ? (float)t[i] : fill;
-    }
-}
 // The value of lane ^ O, without LDS where the hardware has a lane permutation for it.
 template <int O> __device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
     static_assert(O == 1 || O == 2 || O == 4 || O == 8 || O == 16 || O == 32, "one bit");
@@ -109,6 +91,7 @@ template <int O> __device__ __forceinline__ float xor_lane(float v) {
 template <int O> __device__ __forceinline__ unsigned long long xor_lane(unsigned long long v) {
     return (unsigned long long)xor_lane<O>((uint32_t)(v >> 32)) << 32 | xor_lane<O>((uint32_t)v);
 }
+struct LargerWord { __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return max(a, b); } };
 // f over the G lanes (a power of two) of a group, in every lane of it
 template <int G, typename T, typename F> __device__ __forceinline__ T group_all(T v, F f) {
     if constexpr (G > 1) v = f(v, xor_lane<1>(v));

@@ -46,12 +46,13 @@ __global__ __launch_bounds__(64 * FW) void k_linear_direct(LinearArgs a, int yt,
     const uint32_t from = blockIdx.y * k_part, end = a.k - from < k_part ? a.k : from + k_part;
     const uint32_t chunks = (a.k + 63) / 64, pitch = chunks * 64 + 16;
     const uint64_t mine = l0 + 16 * group + lr, l = mine < longer ? mine : longer - 1;
-    const int8_t *pl = (TALL ? static_cast<const int8_t *>(a.x) + (FLOATS ? 0 : l * a.ldx) : a.w + l * a.ldw) + 16 * lq;
+    const int8_t *xc = static_cast<const int8_t *>(a.x);   // (codes)
+    const int8_t *pl = (TALL ? xc + (FLOATS ? 0 : l * a.ldx) : a.w + l * a.ldw) + 16 * lq;
     const int8_t *ps[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const uint64_t r = 16 * m + lr, rr = r < shorter ? r : shorter - 1;
-        ps[m] = (TALL ? a.w + rr * a.ldw : static_cast<const int8_t *>(a.x) + (FLOATS ? 0 : rr * a.ldx)) + 16 * lq;
+        ps[m] = (TALL ? a.w + rr * a.ldw : xc + (FLOATS ? 0 : rr * a.ldx)) + 16 * lq;
     }
     // The wave's u-th block of round t, of `whole` blocks of 64 bytes and then a rest.
     const uint32_t whole = (end - from) / 64;
@@ -133,7 +134,8 @@ __global__ __launch_bounds__(64 * FW) void k_linear_direct(LinearArgs a, int yt,
             if (block(t, u) >= whole) continue;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-                w[m][u] = FLOATS && !TALL ? code(lds_row(m), place(block(t, u))) : load16_at(ps[m] + place(block(t, u)), ODD);
+                w[m][u] = FLOATS && !TALL ? code(lds_row(m), place(block(t, u)))
+                                          : load16_at(ps[m] + place(block(t, u)), ODD);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -205,7 +207,8 @@ static void linear_direct(const LinearArgs &a, const DirectGrid &d, uint32_t lds
     else odd ? go(k_linear_direct<XT, MT, 16, TALL, true>) : go(k_linear_direct<XT, MT, 16, TALL, false>);
 }
 template <int XT>
-static void linear_direct(const LinearArgs &a, uint32_t parts, uint32_t k_part, int32_t *sums, int yt, hipStream_t st) {
+static void linear_direct(const LinearArgs &a, uint32_t parts, uint32_t k_part, int32_t *sums, int yt,
+                          hipStream_t st) {
     constexpr bool FLOATS = XT != FSX_DTYPE_I8;
     const DirectGrid d(a.rows, a.k, a.n, FLOATS);
     const uint32_t groups = (uint32_t)(((d.tall ? a.n : a.rows) + 15) / 16);
@@ -244,9 +247,8 @@ struct TileGrid {
 
 // ---- tiles of BN channels x BM rows, waves of WN x WM, BK bytes of k at a time through LDS
 //
-// The weights are the first operand of v_mfma_i32_32x32x32_i8 and x the second: lane l gives
-// bytes 16 (l / 32) .. of row l % 32 of either, and holds channels 8 j + 4 (l / 32) .. + 3 of
-// row l % 32 of the result: four neighbouring channels of one row.
+// The weights are the first operand of v_mfma_i32_16x16x64_i8 and x the second, as above: a lane
+// holds four neighbouring channels of one row.
 //
 // LDS holds a row's BK bytes as 16-byte chunks, chunk c of row r at place c ^ key(r): sixteen
 // lanes read one chunk of sixteen rows at once, and those of them whose rows share banks (256
@@ -277,7 +279,9 @@ template <int ROWS, int BK, int THREADS, bool DMA> struct Stage {
         odd = (((uintptr_t)p | ld) & 3) != 0;
         const uint32_t last = (uint32_t)(rows - r0 < ROWS ? rows - r0 : ROWS) - 1;
         // raw buffer, 32-bit data; it ends with the chunk that the last row's end lies in
-        if (DMA) buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(base), 0, last * (uint32_t)ld + ((k + 15) & ~15u), 0x00020000);
+        if (DMA)
+            buf = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(base), 0,
+                                                    last * (uint32_t)ld + ((k + 15) & ~15u), 0x00020000);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const uint32_t r = i * STEP + tr, rr = r < last ? r : last;
@@ -314,20 +318,19 @@ template <int ROWS, int BK, int THREADS, bool DMA> struct Stage {
     }
 };
 
-// MF 32: v_mfma_i32_32x32x32_i8, 16: v_mfma_i32_16x16x64_i8.
-template <int MF, int WN, int WM, int BK>
+template <int WN, int WM, int BK>
 struct WaveTile {
-    static constexpr int TN = WN / MF, TM = WM / MF, S = BK * MF / 1024, E = MF * MF / 64;
-    typedef int Acc __attribute__((ext_vector_type(E)));
-    Acc acc[TN][TM];
+    static constexpr int TN = WN / 16, TM = WM / 16, S = BK / 64;
+    v4i acc[TN][TM];
     struct Frag { v4i w[TN], x[TM]; };
     Frag f[2];
-    __device__ __forceinline__ void read(Frag &to, const int8_t *sw, const int8_t *sx, uint32_t wn, uint32_t wm, int s) {
-        const uint32_t lane = __lane_id(), lr = lane % MF, at = ((64 / MF * s + lane / MF) ^ place_key<BK>(lr)) * 16;
+    __device__ __forceinline__ void read(Frag &to, const int8_t *sw, const int8_t *sx, uint32_t wn, uint32_t wm,
+                                         int s) {
+        const uint32_t lane = __lane_id(), lr = lane % 16, at = ((4 * s + lane / 16) ^ place_key<BK>(lr)) * 16;
 #pragma unroll
-        for (int i = 0; i < TN; ++i) to.w[i] = *reinterpret_cast<const v4i *>(sw + (wn + MF * i + lr) * BK + at);
+        for (int i = 0; i < TN; ++i) to.w[i] = *reinterpret_cast<const v4i *>(sw + (wn + 16 * i + lr) * BK + at);
 #pragma unroll
-        for (int j = 0; j < TM; ++j) to.x[j] = *reinterpret_cast<const v4i *>(sx + (wm + MF * j + lr) * BK + at);
+        for (int j = 0; j < TM; ++j) to.x[j] = *reinterpret_cast<const v4i *>(sx + (wm + 16 * j + lr) * BK + at);
     }
     // Step s of a tile from f[s & 1], the next step's reads under way meanwhile.
     template <typename F> __device__ __forceinline__ void step(int s, F next) {
@@ -337,12 +340,8 @@ struct WaveTile {
 #pragma unroll
         for (int i = 0; i < TN; ++i)
 #pragma unroll
-            for (int j = 0; j < TM; ++j) {
-                if constexpr (MF == 32)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[s & 1].w[i], f[s & 1].x[j], acc[i][j], 0, 0, 0);
-                else
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s & 1].w[i], f[s & 1].x[j], acc[i][j], 0, 0, 0);
-            }
+            for (int j = 0; j < TM; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[s & 1].w[i], f[s & 1].x[j], acc[i][j], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     }
 };
@@ -376,19 +375,19 @@ template <int LATER> __device__ __forceinline__ void tile_barrier() {
 
 #endif
 
-// Two buffers: tile i + 1 is loaded while tile i is multiplied. More (DMA): NS - 1 tiles are
+// Two buffers: tile i + 1 is loaded while tile i is multiplied. Four (DMA): three tiles are
 // under way, the next one is in LDS already and its first step's reads are made ahead of the
 // barrier, so that the matrix instructions go on behind it.
 //
 // Few tiles over a long k: block (.., p) takes bytes p k_part .. of k and leaves its sums in
 // `sums` [p][rows][n]; k_linear_join adds the parts.
-template <int MF, int BN, int BM, int WN, int WM, int BK, int NS, bool DMA, int YT>
+template <int BN, int BM, int WN, int WM, int BK, int NS, bool DMA, int YT>
 __global__ __launch_bounds__(BN / WN * (BM / WM) * 64) void k_linear_tile(LinearArgs a, TileGrid tg, uint32_t k_part,
                                                                           int32_t *sums) {
 #ifdef __HIP_DEVICE_COMPILE__
     constexpr int THREADS = BN / WN * (BM / WM) * 64;
-    constexpr bool DEEP = NS > 2;
-    static_assert(DMA || !DEEP, "through registers: two buffers");
+    constexpr bool DEEP = NS == 4;
+    static_assert(NS == 2 || (DEEP && DMA), "two buffers, or four by DMA");
     if constexpr (YT == kSums) {
         const uint32_t from = blockIdx.y * k_part;
         a.x = static_cast<const int8_t *>(a.x) + from;
@@ -397,15 +396,15 @@ __global__ __launch_bounds__(BN / WN * (BM / WM) * 64) void k_linear_tile(Linear
     }
     // (a variable for each buffer: the compiler then knows which loads a read has to wait for)
     constexpr int SIZE = (BN + BM) * BK;
-    __shared__ __attribute__((aligned(16))) int8_t s_0[SIZE], s_1[SIZE], s_2[NS > 2 ? SIZE : 16],
-        s_3[NS > 3 ? SIZE : 16];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane % MF,
-                   part = lane / MF;
+    __shared__ __attribute__((aligned(16))) int8_t s_0[SIZE], s_1[SIZE], s_2[DEEP ? SIZE : 16],
+        s_3[DEEP ? SIZE : 16];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane % 16,
+                   part = lane / 16;
     const uint32_t wn = wave % (BN / WN) * WN, wm = wave / (BN / WN) * WM;
     uint32_t bn, bm;
     tg.place(blockIdx.x, bn, bm);
     const uint64_t n0 = (uint64_t)bn * BN, m0 = (uint64_t)bm * BM;
-    WaveTile<MF, WN, WM, BK> t;
+    WaveTile<WN, WM, BK> t;
     constexpr int S = t.S;
 #pragma unroll
     for (int i = 0; i < t.TN; ++i)
@@ -425,7 +424,7 @@ __global__ __launch_bounds__(BN / WN * (BM / WM) * 64) void k_linear_tile(Linear
         lw.load(to, wave, i * BK, a.k);
         lx.load(to + BN * BK, wave, i * BK, a.k);
     };
-    auto read = [&](typename WaveTile<MF, WN, WM, BK>::Frag &to, const int8_t *from, int s) {
+    auto read = [&](typename WaveTile<WN, WM, BK>::Frag &to, const int8_t *from, int s) {
         t.read(to, from, from + BN * BK, wn, wm, s);
     };
     auto tail = [&](uint32_t i, int8_t *of) {
@@ -461,36 +460,27 @@ __global__ __launch_bounds__(BN / WN * (BM / WM) * 64) void k_linear_tile(Linear
     } else {
         static_assert(S % 2 == 0, "a tile's first step is in f[0]");
         load(1, s_1);
-        if constexpr (NS > 3) load(2, s_2);
-        tile_barrier<(NS - 2) * EACH>();
+        load(2, s_2);
+        tile_barrier<2 * EACH>();
         tail(0, s_0);
         read(t.f[0], s_0, 0);
-        // tile i from `from`; tile i + 1 has arrived in `next`, tile i + NS - 1 goes to `to`, which
+        // tile i from `from`; tile i + 1 has arrived in `next`, tile i + 3 goes to `to`, which
         // held tile i - 1
         auto step = [&](uint32_t i, int8_t *from, int8_t *next, int8_t *to) {
-            tile_barrier<(NS - 3) * EACH>();
+            tile_barrier<EACH>();
             tail(i + 1, next);
-            load(i + NS - 1, to);
+            load(i + 3, to);
             multiply(from, [&](auto &f) { read(f, next, 0); });   // (behind the last tile: unused)
         };
         for (uint32_t i = 0;;) {
-            if constexpr (NS == 3) {
-                step(i, s_0, s_1, s_2);
-                if (++i == tiles) break;
-                step(i, s_1, s_2, s_0);
-                if (++i == tiles) break;
-                step(i, s_2, s_0, s_1);
-                if (++i == tiles) break;
-            } else {
-                step(i, s_0, s_1, s_3);
-                if (++i == tiles) break;
-                step(i, s_1, s_2, s_0);
-                if (++i == tiles) break;
-                step(i, s_2, s_3, s_1);
-                if (++i == tiles) break;
-                step(i, s_3, s_0, s_2);
-                if (++i == tiles) break;
-            }
+            step(i, s_0, s_1, s_3);
+            if (++i == tiles) break;
+            step(i, s_1, s_2, s_0);
+            if (++i == tiles) break;
+            step(i, s_2, s_3, s_1);
+            if (++i == tiles) break;
+            step(i, s_3, s_0, s_2);
+            if (++i == tiles) break;
         }
     }
     if constexpr (YT == kSums) {
@@ -498,46 +488,40 @@ __global__ __launch_bounds__(BN / WN * (BM / WM) * 64) void k_linear_tile(Linear
         for (int i = 0; i < t.TN; ++i)
 #pragma unroll
             for (int j = 0; j < t.TM; ++j) {
-                const uint64_t r = m0 + wm + MF * j + lr, c = n0 + wn + MF * i + 4 * part;
+                const uint64_t r = m0 + wm + 16 * j + lr, c = n0 + wn + 16 * i + 4 * part;
                 if (r >= a.rows) continue;
                 int32_t *to = sums + (blockIdx.y * a.rows + r) * a.n;
 #pragma unroll
-                for (int e = 0; e < t.E; ++e)
-                    if (c + 8 * (e / 4) + e % 4 < a.n) to[c + 8 * (e / 4) + e % 4] = t.acc[i][j][e];
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < a.n) to[c + e] = t.acc[i][j][e];
             }
     } else {
-    using T = typename Elem<YT>::T;
-    // the channels' scales and biases come through LDS
-    float *s_ws = reinterpret_cast<float *>(s_0), *s_b = s_ws + BN;
-    __syncthreads();
-    for (uint32_t c = threadIdx.x; c < BN; c += THREADS) {
-        const uint64_t cc = n0 + c < a.n ? n0 + c : a.n - 1;
-        s_ws[c] = a.w_scale[cc];
-        s_b[c] = a.bias ? a.bias[cc] : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < t.TN; ++i) {
-        const uint32_t cw = wn + MF * i + 4 * part;
-        const int64_t left = (int64_t)a.n - (int64_t)(n0 + cw);   // channels from this lane's first on
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < t.TM; ++j) {
-            const uint64_t r = m0 + wm + MF * j + lr;
-            const float xs = a.x_scale[r < a.rows ? r : a.rows - 1];
-            float v[t.E / 4][4];
-#pragma unroll
-            for (int e = 0; e < t.E; ++e)
-                v[e / 4][e % 4] = scaled(t.acc[i][j][e], xs, s_ws[cw + 8 * (e / 4) + e % 4], s_b[cw + 8 * (e / 4) + e % 4]);
-#pragma unroll
-            for (int g = 0; g < t.E / 4; ++g) activate(v[g], a.act);
-            if (r >= a.rows) continue;
-            T *y = static_cast<T *>(a.y) + r * a.ldy + n0 + cw;
-#pragma unroll
-            for (int g = 0; g < t.E / 4; ++g)
-                if (left > 8 * g) store4(y + 8 * g, v[g], left - 8 * g);
+        using T = typename Elem<YT>::T;
+        // the channels' scales and biases come through LDS
+        float *s_ws = reinterpret_cast<float *>(s_0), *s_b = s_ws + BN;
+        __syncthreads();
+        for (uint32_t c = threadIdx.x; c < BN; c += THREADS) {
+            const uint64_t cc = n0 + c < a.n ? n0 + c : a.n - 1;
+            s_ws[c] = a.w_scale[cc];
+            s_b[c] = a.bias ? a.bias[cc] : 0.0f;
         }
-    }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < t.TN; ++i) {
+            const uint32_t cw = wn + 16 * i + 4 * part;
+            const int64_t left = (int64_t)a.n - (int64_t)(n0 + cw);   // channels from this lane's first on
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < t.TM; ++j) {
+                const uint64_t r = m0 + wm + 16 * j + lr;
+                const float xs = a.x_scale[r < a.rows ? r : a.rows - 1];
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = scaled(t.acc[i][j][e], xs, s_ws[cw + e], s_b[cw + e]);
+                activate(v, a.act);
+                if (r < a.rows && left > 0) store4(static_cast<T *>(a.y) + r * a.ldy + n0 + cw, v, left);
+            }
+        }
     }
 #endif
 }
@@ -565,7 +549,8 @@ static void join_parts(const LinearArgs &a, int yt, uint32_t parts, const int32_
 }
 
 // Rows that the DMA cannot bring into rows that it can, 16 bytes a thread; 0 behind their ends.
-__global__ __launch_bounds__(256) void k_pack_rows(const int8_t *p, uint64_t ld, uint64_t rows, uint32_t k, int8_t *to) {
+__global__ __launch_bounds__(256) void k_pack_rows(const int8_t *p, uint64_t ld, uint64_t rows, uint32_t k,
+                                                   int8_t *to) {
     const uint32_t per = (k + 15) / 16;
     const bool odd = (((uintptr_t)p | ld) & 3) != 0;
     for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < rows * per; i += gridDim.x * 256ull) {
@@ -576,14 +561,14 @@ __global__ __launch_bounds__(256) void k_pack_rows(const int8_t *p, uint64_t ld,
     }
 }
 
-template <int MF, int BN, int BM, int WN, int WM, int BK, int NS, bool DMA>
+template <int BN, int BM, int WN, int WM, int BK, int NS, bool DMA>
 static void linear_tile(const LinearArgs &a, int yt, hipStream_t st) {
     const TileGrid tg((a.n + BN - 1) / BN, (a.rows + BM - 1) / BM);
     constexpr int threads = BN / WN * (BM / WM) * 64;
     auto go = [&](auto kernel) { kernel<<<tg.tiles, threads, 0, st>>>(a, tg, a.k, nullptr); };
-    if (yt == FSX_DTYPE_F32) go(k_linear_tile<MF, BN, BM, WN, WM, BK, NS, DMA, FSX_DTYPE_F32>);
-    else if (yt == FSX_DTYPE_F16) go(k_linear_tile<MF, BN, BM, WN, WM, BK, NS, DMA, FSX_DTYPE_F16>);
-    else go(k_linear_tile<MF, BN, BM, WN, WM, BK, NS, DMA, FSX_DTYPE_BF16>);
+    if (yt == FSX_DTYPE_F32) go(k_linear_tile<BN, BM, WN, WM, BK, NS, DMA, FSX_DTYPE_F32>);
+    else if (yt == FSX_DTYPE_F16) go(k_linear_tile<BN, BM, WN, WM, BK, NS, DMA, FSX_DTYPE_F16>);
+    else go(k_linear_tile<BN, BM, WN, WM, BK, NS, DMA, FSX_DTYPE_BF16>);
 }
 
 // Operands that the DMA can bring: chunks at 16-byte addresses, a tile's rows within 2^31 bytes.
@@ -602,7 +587,8 @@ static bool dma_can(const void *p, uint64_t ld) { return ((uintptr_t)p | ld) % 1
 // Few blocks over a long k are cut into parts; the join is another launch. In tiles: 40 rows of
 // 10931 to 42 channels 14.3 us in 10 parts, 13.3 in 20; through registers more tiles are cut (107
 // rows of 6581 to 6892 channels 57 -> 38) than by DMA (603 rows of 3982 to 1394 22.6 -> 25.9: not).
-// Direct: 14 rows of 11313 to 1384 channels 24 -> 12.8, but one row of 4096 to 1024 channels 4.8 -> 7.1: by the bytes that a block takes.
+// Direct: 14 rows of 11313 to 1384 channels 24 -> 12.8, but one row of 4096 to 1024 channels 4.8 ->
+// 7.1: by the bytes that a block takes.
 // Operands that the DMA cannot bring are packed for it where the work repays the copy: 4096 rows
 // of 4096 to 4096 channels at odd strides 182 -> 78 us, 1006 rows of 8444 to 2643 channels 104 ->
 // 64, but 1000 rows of 1003 to 777 channels 8.0 -> 12.2.
@@ -677,20 +663,20 @@ static void linear_tiles(const LinearArgs &a, int yt, const LinearPlan &ks, void
         const dim3 grid(tg.tiles, ks.parts);
         int32_t *sums = static_cast<int32_t *>(sums_at);
         if (dma_can(a.x, a.ldx) && dma_can(a.w, a.ldw))
-            k_linear_tile<16, 64, 64, 32, 16, 256, 2, true, kSums><<<grid, 512, 0, st>>>(a, tg, ks.k_part, sums);
-        else k_linear_tile<16, 64, 64, 32, 16, 128, 2, false, kSums><<<grid, 512, 0, st>>>(a, tg, ks.k_part, sums);
+            k_linear_tile<64, 64, 32, 16, 256, 2, true, kSums><<<grid, 512, 0, st>>>(a, tg, ks.k_part, sums);
+        else k_linear_tile<64, 64, 32, 16, 128, 2, false, kSums><<<grid, 512, 0, st>>>(a, tg, ks.k_part, sums);
         join_parts(a, yt, ks.parts, sums, st);
         return;
     }
     auto tiles = [&](uint64_t size) { return (a.n + size - 1) / size * ((a.rows + size - 1) / size); };
     if (dma_can(a.x, a.ldx) && dma_can(a.w, a.ldw)) {
-        if (a.n <= 64 && tiles(64) >= 256) linear_tile<16, 64, 64, 32, 16, 128, 2, true>(a, yt, st);
-        else if (a.k > 2048 && tiles(256) >= 256) linear_tile<16, 256, 256, 128, 64, 128, 2, true>(a, yt, st);
-        else if (tiles(128) >= 320) linear_tile<16, 128, 128, 64, 32, 128, 2, true>(a, yt, st);
-        else if (tiles(128) >= 192) linear_tile<16, 128, 128, 64, 32, 128, 4, true>(a, yt, st);
-        else linear_tile<16, 64, 64, 32, 16, 256, 2, true>(a, yt, st);
+        if (a.n <= 64 && tiles(64) >= 256) linear_tile<64, 64, 32, 16, 128, 2, true>(a, yt, st);
+        else if (a.k > 2048 && tiles(256) >= 256) linear_tile<256, 256, 128, 64, 128, 2, true>(a, yt, st);
+        else if (tiles(128) >= 320) linear_tile<128, 128, 64, 32, 128, 2, true>(a, yt, st);
+        else if (tiles(128) >= 192) linear_tile<128, 128, 64, 32, 128, 4, true>(a, yt, st);
+        else linear_tile<64, 64, 32, 16, 256, 2, true>(a, yt, st);
     } else {
-        linear_tile<16, 64, 64, 32, 16, 128, 2, false>(a, yt, st);
+        linear_tile<64, 64, 32, 16, 128, 2, false>(a, yt, st);
     }
 }
 

@@ -17,7 +17,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct Larger { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
 struct LargerFloat { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
-struct LargerWord { __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return max(a, b); } };
 struct PlusWord { __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return a + b; } };
 struct Plus { __device__ float operator()(float a, float b) const { return a + b; } };
 

@@ -142,7 +142,6 @@ template <int DT> struct RawChunk {   // kQV values as they lie in memory
         return v4i{(int)q[0], (int)q[1], (int)q[2], (int)q[3]};
     }
 };
-struct LargerWord { __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return max(a, b); } };
 
 // ---- products
 
