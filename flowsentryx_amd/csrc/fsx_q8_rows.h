@@ -235,9 +235,15 @@ __device__ __forceinline__ void store4(T *p, const float (&v)[4], int64_t ok) {
 }
 
 __device__ __forceinline__ void activate(float (&v)[4], int act) {
-    if (act == FSX_ACT_NONE) return;
+    if (act == FSX_ACT_RELU) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = act == FSX_ACT_RELU ? relu(v[e]) : sigmoid(v[e]);
+        for (int e = 0; e < 4; ++e) v[e] = relu(v[e]);
+    } else if (act == FSX_ACT_SIGMOID) {
+        // (a branch: the compiler would compute it for every activation and then choose, 150 instructions)
+        asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = sigmoid(v[e]);
+    }
 }
 
 // Four neighbouring channels' scales and biases; channels behind the last: the last one's.
