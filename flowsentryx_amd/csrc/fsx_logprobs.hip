@@ -15,8 +15,8 @@ namespace fsx {
 constexpr float kLowest = -3.402823466e38f;   // the maximum of no values: finite, so that -inf - m is -inf
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct Larger { template <typename T> __device__ T operator()(T a, T b) const { return a > b ? a : b; } };
 struct LargerFloat { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct LesserWord { __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return min(a, b); } };
 struct PlusWord { __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return a + b; } };
 struct Plus { __device__ float operator()(float a, float b) const { return a + b; } };
 
@@ -64,7 +64,7 @@ struct Sums {
     __device__ void add(float x) {      // x <= m, or -inf, or NaN
         const float z = x - m, e = exp_of(z);
         s += e;
-        t += fmaxf(z, -200.0f) * e;     // -inf: 0 * -200; NaN goes on through e
+        t = fmaf(fmaxf(z, -200.0f), e, t);   // -inf: 0 * -200; NaN goes on through e
     }
     // the sums of the G lanes of a group, in every lane of it
     template <int G> __device__ void join_group() {
@@ -198,14 +198,16 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
             Alt mine = 0;
             uint64_t to = r * a.top + g;
             for (uint32_t k = 0;; ++k) {
-                uint32_t b = w[0], c = c0;
+                uint32_t b = w[0];
 #pragma unroll
-                for (int i = 1; i < N; ++i)
-                    if (w[i] > b) { b = w[i]; c = c0 + i; }
-                const Alt own = b ? (Alt)b << 32 | (uint32_t)~c : 0;
-                const Alt best = group_all<G>(own, Larger());
+                for (int i = 1; i < N; ++i) b = max(b, w[i]);
+                const uint32_t best = group_all<G>(b, LargerWord());
+                uint32_t c = ~0u;   // its first place
+#pragma unroll
+                for (int i = N - 1; i >= 0; --i) c = w[i] == best ? c0 + i : c;
+                c = group_all<G>(c, LesserWord());
                 const uint32_t place = k % G;
-                if (place == g) mine = best;
+                if (place == g) mine = best ? (Alt)best << 32 | (uint32_t)~c : 0;
                 const bool last = k + 1 == a.top;
                 if (last || place == G - 1) {
                     if (g <= place && live) {
@@ -215,9 +217,8 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
                     if (last) break;
                     to += G;
                 }
-                const uint32_t gone = (uint32_t)~(uint32_t)best;   // (in its own lane one of c0 .. c0 + N - 1)
 #pragma unroll
-                for (int i = 0; i < N; ++i) w[i] = gone == c0 + i ? 0 : w[i];
+                for (int i = 0; i < N; ++i) w[i] = c - c0 == (uint32_t)i ? 0 : w[i];
             }
             continue;
         }
