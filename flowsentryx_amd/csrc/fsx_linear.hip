@@ -181,8 +181,9 @@ struct DirectGrid {
     bool tall;
     uint32_t waves, kw, blocks;
     static uint64_t pitch(uint32_t k) { return (k + 63) / 64 * 64 + 16; }
-    DirectGrid(uint64_t rows, uint32_t k, uint32_t n, bool floats) {
-        tall = n <= rows && !(floats && rows <= kFusedRows);
+    // (the whole product's side: a launch of a part of its rows may hold fewer of them)
+    static bool tall_of(uint64_t rows, uint32_t n, bool floats) { return n <= rows && !(floats && rows <= kFusedRows); }
+    DirectGrid(uint64_t rows, uint32_t k, uint32_t n, bool floats, bool tall) : tall(tall) {
         const uint64_t sixteens = ((tall ? rows : n) + 15) / 16;
         // us of one row, 4096 / 8192 / 16384 channels of 4096: eight waves 6.4 / 9.1 / 16.8, sixteen
         // 5.9 / 10.9 / 20.0
@@ -207,10 +208,10 @@ static void linear_direct(const LinearArgs &a, const DirectGrid &d, uint32_t lds
     else odd ? go(k_linear_direct<XT, MT, 16, TALL, true>) : go(k_linear_direct<XT, MT, 16, TALL, false>);
 }
 template <int XT>
-static void linear_direct(const LinearArgs &a, uint32_t parts, uint32_t k_part, int32_t *sums, int yt,
+static void linear_direct(const LinearArgs &a, bool tall, uint32_t parts, uint32_t k_part, int32_t *sums, int yt,
                           hipStream_t st) {
     constexpr bool FLOATS = XT != FSX_DTYPE_I8;
-    const DirectGrid d(a.rows, a.k, a.n, FLOATS);
+    const DirectGrid d(a.rows, a.k, a.n, FLOATS, tall);
     const uint32_t groups = (uint32_t)(((d.tall ? a.n : a.rows) + 15) / 16);
     const uint32_t lds = FLOATS ? (uint32_t)d.codes_bytes(a.rows, a.k) : 0;
     auto go = [&](auto mt, auto tall) {
@@ -596,7 +597,7 @@ enum LinearForm { kNarrow, kDirectFloats, kDirect, kTiles };
 struct LinearPlan {
     LinearForm form;
     uint32_t parts = 1, k_part;
-    bool pack_x = false, pack_w = false;
+    bool tall = false, pack_x = false, pack_w = false;
     uint64_t codes = 0, x_bytes = 0, w_bytes = 0, sums = 0;   // of the workspace, in this order
     uint64_t bytes() const { return codes + x_bytes + w_bytes + sums; }
 
@@ -614,8 +615,9 @@ struct LinearPlan {
             return;
         }
         if (floats) {
-            const DirectGrid d(rows, k, n, true);
+            const DirectGrid d(rows, k, n, true, DirectGrid::tall_of(rows, n, true));
             const uint64_t lds = d.codes_bytes(rows, k);
+            tall = d.tall;
             if (d.tall ? n <= kDirectMost && lds <= kTallBytes : rows <= kFusedRows && lds <= kFusedBytes) {
                 form = kDirectFloats;
                 return;
@@ -623,7 +625,8 @@ struct LinearPlan {
             codes = code_space(rows, k).bytes;
             x_fits = true;   // (what the quantiser leaves)
         }
-        const DirectGrid d(rows, k, n, false);
+        const DirectGrid d(rows, k, n, false, DirectGrid::tall_of(rows, n, false));
+        tall = d.tall;
         const uint64_t shorter = d.tall ? n : rows, weights = (uint64_t)n * k;
         if (shorter <= kDirectMost && (d.tall || (shorter <= 16 ? weights < 1u << 26 || !w_fits : weights < 1u << 25))) {
             form = kDirect;
@@ -728,9 +731,9 @@ hipError_t launch_linear(const LinearArgs &in, int x_dtype, int y_dtype, void *w
     if (x_dtype != FSX_DTYPE_I8 && (p.form == kNarrow || p.form == kDirectFloats)) {
         slabs(a, y_dtype, elem_size(x_dtype), [&](const LinearArgs &b) {
             if (p.form == kNarrow) launch_linear_narrow(b, x_dtype, y_dtype, st);
-            else if (x_dtype == FSX_DTYPE_F32) linear_direct<FSX_DTYPE_F32>(b, 1, b.k, nullptr, y_dtype, st);
-            else if (x_dtype == FSX_DTYPE_F16) linear_direct<FSX_DTYPE_F16>(b, 1, b.k, nullptr, y_dtype, st);
-            else linear_direct<FSX_DTYPE_BF16>(b, 1, b.k, nullptr, y_dtype, st);
+            else if (x_dtype == FSX_DTYPE_F32) linear_direct<FSX_DTYPE_F32>(b, p.tall, 1, b.k, nullptr, y_dtype, st);
+            else if (x_dtype == FSX_DTYPE_F16) linear_direct<FSX_DTYPE_F16>(b, p.tall, 1, b.k, nullptr, y_dtype, st);
+            else linear_direct<FSX_DTYPE_BF16>(b, p.tall, 1, b.k, nullptr, y_dtype, st);
         });
         return hipGetLastError();
     }
@@ -761,7 +764,7 @@ hipError_t launch_linear(const LinearArgs &in, int x_dtype, int y_dtype, void *w
         if (p.form == kNarrow) launch_linear_narrow(b, FSX_DTYPE_I8, y_dtype, st);
         else if (p.form == kDirect) {
             int32_t *sums = p.parts > 1 ? reinterpret_cast<int32_t *>(at) : nullptr;
-            linear_direct<FSX_DTYPE_I8>(b, p.parts, p.k_part, sums, y_dtype, st);
+            linear_direct<FSX_DTYPE_I8>(b, p.tall, p.parts, p.k_part, sums, y_dtype, st);
             if (sums) join_parts(b, y_dtype, p.parts, sums, st);
         }
         else linear_tiles(b, y_dtype, p, at, st);   // (in parts: small enough for one launch)

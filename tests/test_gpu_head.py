@@ -353,7 +353,7 @@ def test_linear_floats_few_many_channels(head):
 @pytest.mark.parametrize("xt", [*FLOATS, "i8"])
 @pytest.mark.parametrize("rows,k,n", [(9001, 70, 1), (9001, 130, 17), (20005, 300, 32), (140000, 65, 16), (50, 3008, 5),
                                       (50, 3009, 5), (333, 1000, 31), (17, 20000, 9), (40, 7000, 32), (33, 13000, 16),
-                                      (70003, 129, 33), (8200, 520, 12)])
+                                      (70003, 129, 33), (8200, 520, 12), (50, 3008, 20), (8200, 3000, 20)])
 def test_linear_few_channels(head, xt, rows, k, n):
     """Many rows to few channels, at strides that are multiples of 16 and odd ones."""
     g = gen_of("fc", rows, k, n)
@@ -421,6 +421,35 @@ def test_linear_several_launches(head):
         torch.cuda.synchronize()
         assert torch.equal(y, part)
         check_linear(head, x, None, w[-300:], ws[-300:], bias[-300:], "relu", torch.float16)
+
+
+@pytest.mark.parametrize("k,n", [(70, 12), (66, 32), (12, 20)])
+def test_linear_more_rows_than_one_launch(head, k, n):
+    """2^24 rows go in one launch: the few behind them have the bits of a call of their own, and all
+    of one that starts in their midst."""
+    rows = (1 << 24) + 9
+    g = gen_of("slabrows", k, n)
+    w, ws, bias = layer_of(g, n, k, 2, True)
+    layer = head.layer(w, ws, bias, "relu")
+    x = torch.zeros(rows, k, dtype=torch.float16, device="cuda")
+    x[:40] = rows_of(g, 40, k, 0, torch.float16)
+    x[-40:] = rows_of(g, 40, k, 0, torch.float16)
+    x[1 << 23:(1 << 23) + 40] = x[-40:]
+    q, s = torch.empty(rows, k, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    torch.cuda.synchronize()
+    head.quantize(x, q, s)
+    for xx, xs in ((x, None), (q, s)):
+        y = torch.full((rows + 1, n), float(CANARY), dtype=torch.float16, device="cuda")
+        work = head.linear_work(layer, xx)
+        torch.cuda.synchronize()
+        head.linear(layer, xx, xs, y[:rows], work)
+        torch.cuda.synchronize()
+        assert (y[rows] == CANARY).all()
+        assert torch.equal(y[rows - 40:rows], y[1 << 23:(1 << 23) + 40])
+        for part in (slice(0, 40), slice(rows - 40, rows)):
+            z = check_linear(head, xx[part], None if xs is None else xs[part], w, ws, bias, "relu", torch.float16)
+            assert torch.equal(y[part], z)
+        del y, work
 
 
 # ---------------------------------------------------------------- log probabilities
