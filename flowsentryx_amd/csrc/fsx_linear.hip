@@ -159,7 +159,12 @@ __global__ __launch_bounds__(64 * FW) void k_linear_direct(LinearArgs a, int yt,
     for (uint32_t i = wave; i < groups * MT; i += FW) {
         const uint32_t g = i / MT, m = i % MT;
         v4i sum = s_acc[g * kw][m][lane];
-        for (uint32_t q = 1; q < kw; ++q) sum += s_acc[g * kw + q][m][lane];
+        if (kw == FW) {   // (all reads at once)
+#pragma unroll
+            for (int q = 1; q < FW; ++q) sum += s_acc[q][m][lane];
+        } else {
+            for (uint32_t q = 1; q < kw; ++q) sum += s_acc[g * kw + q][m][lane];
+        }
         const uint64_t r = (TALL ? l0 + 16 * g : 16 * m) + lr, c = (TALL ? 16 * m : l0 + 16 * g) + 4 * lq;
         if (r >= a.rows) continue;
         if (!FLOATS && sums) {
