@@ -10,7 +10,8 @@ namespace fsx {
 
 // A group of TPR threads takes a row, up to C chunks of kQV values a thread; they stay in
 // registers between the maximum and the codes (C 0: longer rows are read twice, the second
-// time from cache).
+// time from cache). A row's last chunk ends with the row and repeats codes of the one before, so that
+// rows of kQV values and more are read and written in whole chunks.
 template <int DT, int TPR, int C>
 __global__ __launch_bounds__(256) void k_quantize_rows(const void *__restrict__ xp, uint64_t rows, uint32_t cols,
                                                        uint64_t ldx, int8_t *__restrict__ q, uint64_t ldq,
@@ -23,20 +24,21 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const void *__restrict__ 
         const uint64_t r = r0 + sub;
         const bool live = r < rows;
         const T *x = static_cast<const T *>(xp) + (live ? r : 0) * ldx;
+        auto at = [&](uint32_t c) { return cols >= kQV && c + kQV > cols ? cols - kQV : c; };
         uint32_t m = 0;
         RawChunk<DT> kept[C ? C : 1];
         if constexpr (C > 0) {
 #pragma unroll
             for (int i = 0; i < C; ++i) {
                 const uint32_t c = t * kQV + i * STEP;
-                if (live && c < cols) kept[i].load(x + c, (int64_t)cols - c);
+                if (live && c < cols) kept[i].load(x + at(c), (int64_t)cols - at(c));
             }
 #pragma unroll
             for (int i = 0; i < C; ++i)
                 if (live && t * kQV + i * STEP < cols) m = max(m, kept[i].mag());
         } else if (live) {
             for (uint64_t c = t * kQV; c < cols; c += STEP) {
-                kept[0].load(x + c, (int64_t)cols - (int64_t)c);
+                kept[0].load(x + at((uint32_t)c), (int64_t)cols - at((uint32_t)c));
                 m = max(m, kept[0].mag());
             }
         }
@@ -63,11 +65,11 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const void *__restrict__ 
         if constexpr (C > 0) {
 #pragma unroll
             for (int i = 0; i < C; ++i)
-                if (t * kQV + i * STEP < cols) put(t * kQV + i * STEP, kept[i]);
+                if (t * kQV + i * STEP < cols) put(at(t * kQV + i * STEP), kept[i]);
         } else {
             for (uint64_t c = t * kQV; c < cols; c += STEP) {
-                kept[0].load(x + c, (int64_t)cols - (int64_t)c);
-                put((uint32_t)c, kept[0]);
+                kept[0].load(x + at((uint32_t)c), (int64_t)cols - at((uint32_t)c));
+                put(at((uint32_t)c), kept[0]);
             }
         }
     }
