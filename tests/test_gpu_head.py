@@ -107,6 +107,15 @@ def test_quantize(head, dtype, rows, cols, pad):
     check_quantize(head, rows_of(g, rows, cols, pad, FLOATS[dtype]), pad=(0, 5, 16)[rows % 3])
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("cols", [15, 16, 17, 31, 33, 47, 63, 65, 95, 112, 113, 129, 200, 225, 257, 317, 511, 513, 1000, 1025,
+                                  2000, 2049, 4095, 4097, 8191, 8193, 16383, 16400])
+def test_quantize_row_ends(head, dtype, cols):
+    """Every number of threads and chunks a row, the last chunk beginning inside the one before."""
+    for rows, pad in ((1, 0), (67, 1), (300, 16)):
+        check_quantize(head, rows_of(gen_of("qe", rows, cols), rows, cols, pad, FLOATS[dtype]), pad=pad)
+
+
 def test_quantize_borders(head):
     """Quotients on a half and a last place beside it, for scales with all kinds of last places."""
     g = gen_of("borders")
