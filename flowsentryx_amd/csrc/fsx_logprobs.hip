@@ -117,12 +117,27 @@ __device__ void finish_row(const LogprobArgs &a, uint64_t r, const Sums &q, Alt 
     }
 }
 
+// The upper 12 bits of the n-th largest of a wave's words, from ballots: when
+// they are logits of different places, no logit below it is among the n largest.
+template <int WORDS> __device__ uint32_t nth_largest(const uint32_t (&w)[WORDS], uint32_t n) {
+    uint32_t f = 0;
+#pragma unroll 1
+    for (uint32_t bit = 0x80000000u; bit >= 0x100000u; bit >>= 1) {
+        uint32_t count = 0;
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) count += (uint32_t)__popcll(__ballot(w[i] >= (f | bit)));
+        if (count >= n) f |= bit;
+    }
+    return f;
+}
+
 // ---------------------------------------------------------------- short rows: G lanes a row
 
 // A wave's RW rows: up to KEEP alternatives of each in falling order, and for RANK their words.
-enum { kKeep, kRank, kChoose };   // how a row's alternatives are put in order
-template <int RW, int KEEP, int PITCH> struct ShortRows {
+enum { kKeep, kRank, kChoose, kBound };   // how a row's alternatives are put in order
+template <int RW, int KEEP, int PITCH, int POOL> struct ShortRows {
     Alt alts[RW * KEEP];
+    Alt pool[POOL ? POOL : 1];   // kBound: the rows' candidates
     uint32_t words[PITCH ? RW * PITCH : 4];
     float2 end[RW];    // m, and log S (a bad row: NaN)
     uint32_t found[RW];
@@ -136,16 +151,18 @@ __device__ __forceinline__ void wave_sync() {
 
 // Up to 64 N classes: a lane holds N neighbouring logits of its row, G lanes (a power of two)
 // a row, so the row is read once and its maximum is known before the sums. A wave's alternatives
-// are ordered in LDS and then stored side by side, all its rows' at once. Their order: RANK counts
-// for each logit the ones before it, against the row's words from LDS; else the group's largest
-// word is the next one, and the first lane that holds it clears it. WHOLE: the classes are a
+// are ordered in LDS and then stored side by side, all its rows' at once. Their order: kRank counts
+// for each logit the ones before it, against the row's words from LDS; kBound first leaves out what
+// cannot be one, and counts among the others; kChoose takes the group's largest word as the next
+// one, and the first lane that holds it clears it; kKeep does so in registers. WHOLE: the classes are a
 // multiple of N, so a lane has all of its logits or none; the next rows are then under way while
 // a block works on the ones before.
 template <int DT, int N, int G, bool WHOLE, int ORDER>
 __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t top_inv) {
     using T = typename Elem<DT>::T;
     constexpr uint32_t PER = 256 / G, RW = 64 / G, KEEP = G * N < 64 ? G * N : 64, PITCH = G * N + 4;
-    __shared__ __attribute__((aligned(16))) ShortRows<RW, KEEP, (ORDER == kRank && G > 1 ? PITCH : 0)> s_rows[4];
+    __shared__ __attribute__((aligned(16))) ShortRows<RW, KEEP, (ORDER == kRank && G > 1 ? PITCH : 0),
+                                                    (ORDER == kBound ? 64 * N : 0)> s_rows[4];
     auto &sh = s_rows[threadIdx.x >> 6];
     const uint32_t g = threadIdx.x % G, c0 = g * N;
     const uint64_t step = (uint64_t)gridDim.x * PER;
@@ -267,8 +284,47 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
             }
             found = group_all<G>(found, PlusWord());
         } else {
-            const uint32_t most = a.top < a.v ? a.top : a.v;
-            const uint64_t before = ((1ull << lane) - 1) & ~((1ull << (lane & ~(uint32_t)(G - 1))) - 1);   // of the group
+            const uint64_t group = G == 64 ? ~0ull : ((1ull << G % 64) - 1) << (lane & ~(uint32_t)(G - 1));
+            const uint64_t before = group & ((1ull << lane) - 1);   // lanes of the group
+            uint32_t most = a.top < a.v ? a.top : a.v;
+            if constexpr (ORDER == kBound) {
+                // what is below the top-th largest of the lanes' largest words is no alternative
+                uint32_t b[1] = {w[0]};
+#pragma unroll
+                for (int i = 1; i < N; ++i) b[0] = max(b[0], w[i]);
+                uint32_t low = 0, n = 0;
+                if constexpr (G == 64) {
+                    low = nth_largest(b, a.top);
+                } else {
+#pragma unroll 1
+                    for (uint32_t bit = 0x80000000u; bit >= 0x100000u; bit >>= 1)
+                        if ((uint32_t)__popcll(__ballot(b[0] >= (low | bit)) & group) >= a.top) low |= bit;
+                }
+                low = max(low, 1u);
+                Alt *pool = sh.pool + row * (G * N);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const uint64_t m = __ballot(w[i] >= low);
+                    if (w[i] >= low) pool[n + (uint32_t)__popcll(m & before)] = (Alt)w[i] << 32 | (uint32_t)~(c0 + i);
+                    n += (uint32_t)__popcll(m & group);
+                }
+                wave_sync();
+                if (__ballot(n > 2 * G) == 0) {   // (else one by one)
+                    const Alt x0 = g < n ? pool[g] : 0, x1 = g + G < n ? pool[g + G] : 0;
+                    const uint32_t longest = G == 64 ? n : group_all<64>(n, LargerWord());
+                    uint32_t r0 = 0, r1 = 0;
+#pragma unroll 4
+                    for (uint32_t i = 0; i < longest; ++i) {
+                        const Alt o = i < n ? pool[i] : 0;
+                        r0 += o > x0 ? 1 : 0;
+                        r1 += o > x1 ? 1 : 0;
+                    }
+                    if (x0 && r0 < a.top) to[r0] = x0;
+                    if (x1 && r1 < a.top) to[r1] = x1;
+                    found = n < a.top ? n : a.top;
+                    most = 0;
+                }
+            }
 #pragma unroll 1
             for (uint32_t k = 0; k < most; ++k) {
                 uint32_t b = w[0];
@@ -334,6 +390,16 @@ template <int DT, int N, int G> static bool logprobs_short(const LogprobArgs &a,
             return true;
         }
     }
+    // Bounding costs the same for any number, if there are lanes enough for a bound (us of 20000 bf16 rows of
+    // 500, 5 / 12 / 20 asked for: bounded 21.5 / 22.9 / 24.6, chosen 22.7 / 33.3 / 46.8; of 200, half a wave a row: 11.9 /
+    // 13.4 / 17.5 and 10.3 / 15.2 / 20.9, with 24 of 25 lanes 28.0 and 23.9; a quarter of a wave gains nothing).
+    if constexpr (G >= 32) {
+        if (a.top >= (G == 64 ? 4 : 9) && 8 * ((a.v + N - 1) / N) >= 9 * a.top) {
+            if (a.v % N == 0) go(k_logprobs_short<DT, N, G, true, kBound>);
+            else go(k_logprobs_short<DT, N, G, false, kBound>);
+            return true;
+        }
+    }
     if (a.v % N == 0) go(k_logprobs_short<DT, N, G, true, kChoose>);
     else go(k_logprobs_short<DT, N, G, false, kChoose>);
     return true;
@@ -342,16 +408,11 @@ template <int DT, int N, int G> static bool logprobs_short(const LogprobArgs &a,
 // 20 alternatives 10.4 / 20 us at 16 logits a lane, 9.9 / 11.2 there; of 1004: 13.3 / 23 and 9.6 / 11.2)
 constexpr uint32_t kShort = 64 * 8;
 constexpr uint64_t kManyRows = 1024;   // for long rows: blocks of four waves from here on
+constexpr uint32_t kPool = 128;       // a wave's candidates: 64 alternatives and one of every lane
 constexpr uint32_t kFewTop = 32;       // up to here a bound from 64 words does; beyond, from 256
-// Of the longer of these rows, more than a few alternatives are sooner found by a block that bounds
-// them, if it has lanes enough for the bound (us with 5 / 20 / 64 of 500 logits, 1500 rows: 5.6 / 10.5 /
-// 24.9 here, 6.6 / 7.1 / 47.6 there; 20000 rows: 23 / 48 / 124 and 43 / 48 / 439).
-static bool is_short(uint64_t rows, uint32_t v, uint32_t top) {
-    return v <= kShort && (v <= 128 || top <= (rows <= 2048 ? 5 : 20) || v < (top > kFewTop ? 15 : 10) * top);
-}
 template <int DT> static bool logprobs_short(const LogprobArgs &a, hipStream_t st) {
     constexpr int N = DT == FSX_DTYPE_F32 ? 4 : 8;
-    if (!is_short(a.rows, a.v, a.top)) return false;
+    if (a.v > kShort) return false;
     if (a.v <= 1 * N) return logprobs_short<DT, N, 1>(a, st);
     if (a.v <= 2 * N) return logprobs_short<DT, N, 2>(a, st);
     if (a.v <= 4 * N) return logprobs_short<DT, N, 4>(a, st);
@@ -370,24 +431,9 @@ constexpr uint32_t kMaxParts = 64;
 // The wave's number in its block, as the scalar that it is.
 __device__ __forceinline__ uint32_t wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-// The upper 12 bits of the n-th largest of the waves' words, by each wave from ballots: when
-// they are logits of different places, no logit below it is among the n largest.
-template <int WORDS> __device__ uint32_t nth_largest(const uint32_t (&w)[WORDS], uint32_t n) {
-    uint32_t f = 0;
-#pragma unroll 1
-    for (uint32_t bit = 0x80000000u; bit >= 0x100000u; bit >>= 1) {
-        uint32_t count = 0;
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) count += (uint32_t)__popcll(__ballot(w[i] >= (f | bit)));
-        if (count >= n) f |= bit;
-    }
-    return f;
-}
-
 // Candidates for a row's alternatives: each wave collects its own, unordered; an order comes
 // from counting for each how many are larger (their words all differ), so no list is kept
 // sorted and no lane waits for another.
-constexpr uint32_t kPool = 128;   // a wave's candidates: 64 alternatives and one of every lane
 template <int W> struct Shared {
     Alt pool[W][kPool];
     Alt all[W * kPool];

@@ -570,7 +570,7 @@ def test_logprobs_orders(head, rows, classes, top):
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("rows", [1, 70, 300, 1100])
 @pytest.mark.parametrize("classes,top", [(3, 4), (4, 64), (7, 28), (8, 4), (9, 9), (16, 5), (20, 22), (25, 4), (33, 33),
-                                         (64, 4), (84, 19), (129, 6), (129, 12), (130, 64), (256, 25), (278, 30), (513, 6),
+                                         (64, 4), (84, 19), (100, 20), (128, 32), (200, 20), (200, 23), (256, 9), (300, 33), (500, 55), (512, 64), (129, 6), (129, 12), (130, 64), (256, 25), (278, 30), (513, 6),
                                          (520, 40), (700, 46), (1000, 64), (1004, 20), (1023, 7)])
 def test_logprobs_short_orders(head, dtype, rows, classes, top):
     """Each way that the alternatives of short rows are put in order: ties, masked and empty rows,
