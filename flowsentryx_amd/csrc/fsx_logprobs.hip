@@ -171,13 +171,15 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
     T next[N];
     int32_t next_target = -1;
     auto fetch = [&](uint64_t row) {
-        if (a.target) next_target = a.target[row < a.rows ? row : a.rows - 1];
-        const T *p = static_cast<const T *>(a.x) + (row < a.rows ? row : a.rows - 1) * a.ld + (in_row ? c0 : 0);
+        const uint64_t rr = row < a.rows ? row : a.rows - 1;
+        if (a.target) next_target = a.target[rr];
+        const T *p = static_cast<const T *>(a.x) + rr * a.ld + (in_row ? c0 : 0);
         if constexpr (WHOLE) {
             __builtin_memcpy(next, p, sizeof(next));
         } else {
-            const int64_t ok = (int64_t)a.v - c0;
-            if (ok >= N) __builtin_memcpy(next, p, sizeof(next));
+            // (what follows a row's end up to the last row's can be read; it does not count)
+            const int64_t ok = (int64_t)a.v - (in_row ? c0 : 0), there = (int64_t)((a.rows - 1 - rr) * a.ld) + ok;
+            if (there >= N) __builtin_memcpy(next, p, sizeof(next));
             else
 #pragma unroll
                 for (int i = 0; i < N; ++i) next[i] = p[i < ok ? i : 0];
@@ -404,23 +406,27 @@ template <int DT, int N, int G> static bool logprobs_short(const LogprobArgs &a,
     else go(k_logprobs_short<DT, N, G, false, kChoose>);
     return true;
 }
-// 16 bytes a lane as far as 64 lanes reach (3000 rows of 600 logits and up are faster in blocks: with 3 /
-// 20 alternatives 10.4 / 20 us at 16 logits a lane, 9.9 / 11.2 there; of 1004: 13.3 / 23 and 9.6 / 11.2)
+// Eight logits a lane as far as 64 lanes reach; longer rows are faster in blocks (3000 rows of 600, 3 / 20
+// alternatives 10.4 / 20 us at 16 logits a lane, 9.9 / 11.2 in blocks; of 1004: 13.3 / 23 and 9.6 / 11.2).
 constexpr uint32_t kShort = 64 * 8;
 constexpr uint64_t kManyRows = 1024;   // for long rows: blocks of four waves from here on
 constexpr uint32_t kPool = 128;       // a wave's candidates: 64 alternatives and one of every lane
 constexpr uint32_t kFewTop = 32;       // up to here a bound from 64 words does; beyond, from 256
 template <int DT> static bool logprobs_short(const LogprobArgs &a, hipStream_t st) {
-    constexpr int N = DT == FSX_DTYPE_F32 ? 4 : 8;
     if (a.v > kShort) return false;
-    if (a.v <= 1 * N) return logprobs_short<DT, N, 1>(a, st);
-    if (a.v <= 2 * N) return logprobs_short<DT, N, 2>(a, st);
-    if (a.v <= 4 * N) return logprobs_short<DT, N, 4>(a, st);
-    if (a.v <= 8 * N) return logprobs_short<DT, N, 8>(a, st);
-    if (a.v <= 16 * N) return logprobs_short<DT, N, 16>(a, st);
-    if (a.v <= 32 * N) return logprobs_short<DT, N, 32>(a, st);
-    if (a.v <= 64 * N) return logprobs_short<DT, N, 64>(a, st);
-    return logprobs_short<DT, 8, 64>(a, st);   // (f32: 32 bytes a lane)
+    // 32-bit logits four a lane where half the lanes would do nothing, or where a bound needs more of them
+    // (2^22 rows of 16, 1 / 3 alternatives: 93 / 114 us, eight a lane 76 / 98; 50000 of 200, 3 / 30: 29 / 42 and 18 / 70)
+    if constexpr (DT == FSX_DTYPE_F32) {
+        if (a.v <= 4) return logprobs_short<DT, 4, 1>(a, st);
+        if (a.v > 128 && a.v <= 256 && a.top > 8) return logprobs_short<DT, 4, 64>(a, st);
+    }
+    if (a.v <= 8) return logprobs_short<DT, 8, 1>(a, st);
+    if (a.v <= 16) return logprobs_short<DT, 8, 2>(a, st);
+    if (a.v <= 32) return logprobs_short<DT, 8, 4>(a, st);
+    if (a.v <= 64) return logprobs_short<DT, 8, 8>(a, st);
+    if (a.v <= 128) return logprobs_short<DT, 8, 16>(a, st);
+    if (a.v <= 256) return logprobs_short<DT, 8, 32>(a, st);
+    return logprobs_short<DT, 8, 64>(a, st);
 }
 
 // ---------------------------------------------------------------- long rows: blocks of W waves
