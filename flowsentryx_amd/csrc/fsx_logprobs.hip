@@ -168,17 +168,20 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
     const uint64_t step = (uint64_t)gridDim.x * PER;
     uint64_t r = (uint64_t)blockIdx.x * PER + threadIdx.x / G;
     const bool in_row = c0 < a.v;
+    // the class of the lane's first logit: the last lanes begin so early that they end with the row, and
+    // what belongs to the lane before does not count (G > 1: a row has N logits at least)
+    const uint32_t cb = !WHOLE && G > 1 && c0 > a.v - N ? a.v - N : c0;
     T next[N];
     int32_t next_target = -1;
     auto fetch = [&](uint64_t row) {
         const uint64_t rr = row < a.rows ? row : a.rows - 1;
         if (a.target) next_target = a.target[rr];
-        const T *p = static_cast<const T *>(a.x) + rr * a.ld + (in_row ? c0 : 0);
-        if constexpr (WHOLE) {
+        const T *p = static_cast<const T *>(a.x) + rr * a.ld + (!WHOLE && G > 1 ? cb : in_row ? c0 : 0);
+        if constexpr (WHOLE || G > 1) {
             __builtin_memcpy(next, p, sizeof(next));
         } else {
             // (what follows a row's end up to the last row's can be read; it does not count)
-            const int64_t ok = (int64_t)a.v - (in_row ? c0 : 0), there = (int64_t)((a.rows - 1 - rr) * a.ld) + ok;
+            const int64_t ok = (int64_t)a.v, there = (int64_t)((a.rows - 1 - rr) * a.ld) + ok;
             if (there >= N) __builtin_memcpy(next, p, sizeof(next));
             else
 #pragma unroll
@@ -191,7 +194,7 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
         const bool live = r < a.rows;
         float x[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = (WHOLE ? in_row : c0 + i < a.v) ? (float)next[i] : -INFINITY;
+        for (int i = 0; i < N; ++i) x[i] = (WHOLE ? in_row : G > 1 ? cb + i >= c0 : c0 + i < a.v) ? (float)next[i] : -INFINITY;
         const int32_t target = next_target;
         fetch(r + step);
         Sums q;
@@ -206,7 +209,7 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
         const RowEnd end(q);
         float xt = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < N; ++i) xt = target == (int32_t)(c0 + i) ? x[i] : xt;
+        for (int i = 0; i < N; ++i) xt = target == (int32_t)(cb + i) ? fmaxf(xt, x[i]) : xt;
         xt = group_all<G>(xt, LargerFloat());
         if (live && g == 0) put_row(a, r, end, target, xt);
         if (a.top == 0) continue;
@@ -223,7 +226,7 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
                 const uint32_t best = group_all<G>(b, LargerWord());
                 uint32_t c = ~0u;   // its first place
 #pragma unroll
-                for (int i = N - 1; i >= 0; --i) c = w[i] == best ? c0 + i : c;
+                for (int i = N - 1; i >= 0; --i) c = w[i] == best ? cb + i : c;
                 c = group_all<G>(c, LesserWord());
                 const uint32_t place = k % G;
                 if (place == g) mine = best ? (Alt)best << 32 | (uint32_t)~c : 0;
@@ -237,7 +240,7 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
                     to += G;
                 }
 #pragma unroll
-                for (int i = 0; i < N; ++i) w[i] = c - c0 == (uint32_t)i ? 0 : w[i];
+                for (int i = 0; i < N; ++i) w[i] = c - cb == (uint32_t)i ? 0 : w[i];
             }
             continue;
         }
@@ -259,13 +262,14 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
                         rank[i] += before ? 0 : 1;
                     }
             } else {
-                uint32_t *words = sh.words + row * PITCH;
+                uint32_t *words = sh.words + row * PITCH;   // (in the classes' order, if not at their places)
+                const uint32_t end_word = (a.v + N - 1) / N * N;
 #pragma unroll
                 for (int i = 0; i < N; i += 4)
                     *reinterpret_cast<uint4 *>(words + c0 + i) = uint4{w[i], w[i + 1], w[i + 2], w[i + 3]};
                 wave_sync();
 #pragma unroll 1
-                for (uint32_t j = 0; j < a.v; j += 4) {
+                for (uint32_t j = 0; j < end_word; j += 4) {
                     const uint4 o4 = *reinterpret_cast<const uint4 *>(words + j);
                     const uint32_t o[4] = {o4.x, o4.y, o4.z, o4.w}, ties = j < c0 ? 1 : 0;   // (equal: the lower class)
 #pragma unroll
@@ -282,7 +286,7 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 found += w[i] ? 1 : 0;
-                if (w[i] && rank[i] < a.top) to[rank[i]] = (Alt)w[i] << 32 | (uint32_t)~(c0 + i);
+                if (w[i] && rank[i] < a.top) to[rank[i]] = (Alt)w[i] << 32 | (uint32_t)~(cb + i);
             }
             found = group_all<G>(found, PlusWord());
         } else {
@@ -307,7 +311,7 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const uint64_t m = __ballot(w[i] >= low);
-                    if (w[i] >= low) pool[n + (uint32_t)__popcll(m & before)] = (Alt)w[i] << 32 | (uint32_t)~(c0 + i);
+                    if (w[i] >= low) pool[n + (uint32_t)__popcll(m & before)] = (Alt)w[i] << 32 | (uint32_t)~(cb + i);
                     n += (uint32_t)__popcll(m & group);
                 }
                 wave_sync();
@@ -337,12 +341,12 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
                 found += best ? 1 : 0;
                 const uint64_t holders = __ballot(b == best);
                 if (b == best && best && !(holders & before)) {
-                    uint32_t c = c0;
+                    uint32_t c = cb;
                     bool gone = false;
 #pragma unroll
                     for (int i = 0; i < N; ++i) {
                         const bool it = !gone && w[i] == best;
-                        c = it ? c0 + i : c;
+                        c = it ? cb + i : c;
                         w[i] = it ? 0 : w[i];
                         gone = gone || it;
                     }
