@@ -149,7 +149,7 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Up to 64 N classes: a lane holds N neighbouring logits of its row, G lanes (a power of two)
+// Up to G N classes: a lane holds N neighbouring logits of its row, G lanes (a power of two)
 // a row, so the row is read once and its maximum is known before the sums. A wave's alternatives
 // are ordered in LDS and then stored side by side, all its rows' at once. Their order: kRank counts
 // for each logit the ones before it, against the row's words from LDS; kBound first leaves out what
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
     using T = typename Elem<DT>::T;
     constexpr uint32_t PER = 256 / G, RW = 64 / G, KEEP = G * N < 64 ? G * N : 64, PITCH = G * N + 4;
     __shared__ __attribute__((aligned(16))) ShortRows<RW, KEEP, (ORDER == kRank && G > 1 ? PITCH : 0),
-                                                    (ORDER == kBound ? 64 * N : 0)> s_rows[4];
+                                                    (ORDER == kBound ? 2 * 64 : 0)> s_rows[4];
     auto &sh = s_rows[threadIdx.x >> 6];
     const uint32_t g = threadIdx.x % G, c0 = g * N;
     const uint64_t step = (uint64_t)gridDim.x * PER;
@@ -307,11 +307,12 @@ __global__ __launch_bounds__(256) void k_logprobs_short(LogprobArgs a, uint32_t 
                         if ((uint32_t)__popcll(__ballot(b[0] >= (low | bit)) & group) >= a.top) low |= bit;
                 }
                 low = max(low, 1u);
-                Alt *pool = sh.pool + row * (G * N);
+                Alt *pool = sh.pool + row * (2 * G);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const uint64_t m = __ballot(w[i] >= low);
-                    if (w[i] >= low) pool[n + (uint32_t)__popcll(m & before)] = (Alt)w[i] << 32 | (uint32_t)~(cb + i);
+                    const uint32_t place = n + (uint32_t)__popcll(m & before);
+                    if (w[i] >= low && place < 2 * G) pool[place] = (Alt)w[i] << 32 | (uint32_t)~(cb + i);
                     n += (uint32_t)__popcll(m & group);
                 }
                 wave_sync();
@@ -410,14 +411,19 @@ template <int DT, int N, int G> static bool logprobs_short(const LogprobArgs &a,
     else go(k_logprobs_short<DT, N, G, false, kChoose>);
     return true;
 }
-// Eight logits a lane as far as 64 lanes reach; longer rows are faster in blocks (3000 rows of 600, 3 / 20
-// alternatives 10.4 / 20 us at 16 logits a lane, 9.9 / 11.2 in blocks; of 1004: 13.3 / 23 and 9.6 / 11.2).
+// Eight logits a lane as far as 64 lanes reach, then sixteen, unless more alternatives are asked for than
+// its lanes can bound; else in blocks (20000 bf16 rows of 1004, 1 / 5 / 20 alternatives 18 / 24 / 29 us, in
+// blocks 40 / 43 / 49; 40 of 600, one by one: 127 and 63). 32 a lane leave too few waves (31582 rows of 1279, 1 / 5 / 20:
+// 48 / 86 / 95, in blocks 62 / 68 / 78).
 constexpr uint32_t kShort = 64 * 8;
 constexpr uint64_t kManyRows = 1024;   // for long rows: blocks of four waves from here on
 constexpr uint32_t kPool = 128;       // a wave's candidates: 64 alternatives and one of every lane
 constexpr uint32_t kFewTop = 32;       // up to here a bound from 64 words does; beyond, from 256
 template <int DT> static bool logprobs_short(const LogprobArgs &a, hipStream_t st) {
-    if (a.v > kShort) return false;
+    if (a.v > kShort) {
+        if (a.v > 1024 || (a.top > 3 && 8 * ((a.v + 15) / 16) < 9 * a.top)) return false;
+        return logprobs_short<DT, 16, 64>(a, st);
+    }
     // 32-bit logits four a lane where half the lanes would do nothing, or where a bound needs more of them
     // (2^22 rows of 16, 1 / 3 alternatives: 93 / 114 us, eight a lane 76 / 98; 50000 of 200, 3 / 30: 29 / 42 and 18 / 70)
     if constexpr (DT == FSX_DTYPE_F32) {
