@@ -412,7 +412,7 @@ template <int DT, int N, int G> static bool logprobs_short(const LogprobArgs &a,
     return true;
 }
 // Eight logits a lane as far as 64 lanes reach, then sixteen, unless more alternatives are asked for than
-// its lanes can bound; else in blocks (20000 bf16 rows of 1004, 1 / 5 / 20 alternatives 18 / 24 / 29 us, in
+// its lanes can bound; else in blocks (20000 bf16 rows of 1004, 1 / 5 / 20 alternatives 19 / 27 / 30 us, in
 // blocks 40 / 43 / 49; 40 of 600, one by one: 127 and 63). 32 a lane leave too few waves (31582 rows of 1279, 1 / 5 / 20:
 // 48 / 86 / 95, in blocks 62 / 68 / 78).
 constexpr uint32_t kShort = 64 * 8;
