@@ -184,7 +184,8 @@ __global__ __launch_bounds__(64 * FW) void k_linear_direct(LinearArgs a, int yt,
 // The shape of such a product's launch.
 struct DirectGrid {
     bool tall;
-    uint32_t waves, kw, blocks;
+    uint32_t waves, kw;
+    uint64_t blocks;   // (of all rows; a launch has few enough for a grid)
     static uint64_t pitch(uint32_t k) { return (k + 63) / 64 * 64 + 16; }
     // (the whole product's side: a launch of a part of its rows may hold fewer of them)
     static bool tall_of(uint64_t rows, uint32_t n, bool floats) { return n <= rows && !(floats && rows <= kFusedRows); }
@@ -198,7 +199,7 @@ struct DirectGrid {
         while (kw > 1 && k < 256 * kw && sixteens * kw / waves >= 512 &&
                !(floats && tall && waves / kw * 2 * 16 * pitch(k) > kFusedBytes))
             kw /= 2;
-        blocks = (uint32_t)((sixteens * kw + waves - 1) / waves);
+        blocks = (sixteens * kw + waves - 1) / waves;
     }
     uint64_t codes_bytes(uint64_t rows, uint32_t k) const { return pitch(k) * (tall ? waves / kw * 16 : rows); }
 };
@@ -207,7 +208,7 @@ static void linear_direct(const LinearArgs &a, const DirectGrid &d, uint32_t lds
                           int32_t *sums, int yt, hipStream_t st) {
     const bool odd = (((uintptr_t)a.w | a.ldw) & 3) || (XT == FSX_DTYPE_I8 && (((uintptr_t)a.x | a.ldx) & 3));
     auto go = [&](auto kernel) {
-        kernel<<<dim3(d.blocks, parts), 64 * d.waves, lds, st>>>(a, yt, d.kw, k_part, sums);
+        kernel<<<dim3((uint32_t)d.blocks, parts), 64 * d.waves, lds, st>>>(a, yt, d.kw, k_part, sums);
     };
     if (d.waves == 8) odd ? go(k_linear_direct<XT, MT, 8, TALL, true>) : go(k_linear_direct<XT, MT, 8, TALL, false>);
     else odd ? go(k_linear_direct<XT, MT, 16, TALL, true>) : go(k_linear_direct<XT, MT, 16, TALL, false>);

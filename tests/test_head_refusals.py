@@ -113,6 +113,15 @@ def test_linear_takes_the_workspace_it_asks_for(fake, native):
         assert b"workspace" not in lib.fsx_last_error(ctx), (rows, k, n, xt, ldx, ldw, at, lib.fsx_last_error(ctx))
 
 
+@pytest.mark.parametrize("rows", [(1 << 36) - 16, 1 << 36, (1 << 36) + 16, 1 << 37, (1 << 40) - 16, 1 << 40])
+def test_linear_workspace_of_many_rows(fake, native, rows):
+    """Row counts whose blocks pass 32 bits: the size is worked out, and a product over so many
+    rows is cut into no parts (codes need nothing, floats their codes and scales)."""
+    layer = native.q8_linear(P, P, None, 16384, 16)
+    assert native.linear_q8_work(layer, native.DTYPE_I8, rows) == 0
+    assert native.linear_q8_work(layer, native.DTYPE_F32, rows) == rows * (16384 + 4)
+
+
 def logp(fake, work=0, work_bytes=0, **over):
     a = dict(x=P, dtype=0, rows=4, classes=50, ld=50, target=P, logprob=P, entropy=P, top=3, ids=P, lps=P)
     a.update(over)
