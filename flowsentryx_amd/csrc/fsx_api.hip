@@ -1747,10 +1747,16 @@ int fsx_quantize_rows_device(fsx_ctx *c, const void *d_x, int x_dtype, size_t ro
 static bool layer_sizes_ok(const fsx_q8_linear *l) {
     return l && l->in_features >= 1 && l->in_features <= kMaxIn && l->out_features <= kMaxDim;
 }
+static bool layer_activation_ok(const fsx_q8_linear *l) {
+    return l->activation >= FSX_ACT_NONE && l->activation <= FSX_ACT_SIGMOID && !l->reserved;
+}
 
 size_t fsx_linear_q8_work(const fsx_q8_linear *layer, int x_dtype, size_t rows) {
     if (!layer_sizes_ok(layer) || rows == 0 || rows > kMaxRows || layer->out_features == 0) return 0;
     if (x_dtype != FSX_DTYPE_I8 && !float_type(x_dtype)) return 0;
+    if (!layer_activation_ok(layer) || layer->ld_weight < layer->in_features ||
+        layer->ld_weight > kMaxBytes / layer->out_features)
+        return 0;
     return linear_work(rows, (uint32_t)layer->in_features, (uint32_t)layer->out_features, x_dtype, nullptr, 0,
                        layer->weight, layer->ld_weight);
 }
@@ -1763,7 +1769,7 @@ int fsx_linear_q8_device(fsx_ctx *c, const fsx_q8_linear *layer, const void *d_x
     if (!layer_sizes_ok(layer))
         return set_err(c, -EINVAL, "a layer of %llu to %llu features", (unsigned long long)layer->in_features,
                        (unsigned long long)layer->out_features);
-    if (layer->activation < FSX_ACT_NONE || layer->activation > FSX_ACT_SIGMOID || layer->reserved)
+    if (!layer_activation_ok(layer))
         return set_err(c, -EINVAL, "unknown activation %d", layer->activation);
     if (x_dtype != FSX_DTYPE_I8 && !float_type(x_dtype)) return set_err(c, -EINVAL, "x of type %d", x_dtype);
     if (!float_type(y_dtype)) return set_err(c, -EINVAL, "y of type %d: F32, F16 or BF16", y_dtype);

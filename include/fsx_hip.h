@@ -346,8 +346,8 @@ typedef struct fsx_q8_linear {
     int32_t activation;          /* FSX_ACT_* */
     uint32_t reserved;           /* 0 */
 } fsx_q8_linear;
-/* Workspace bytes of the call below (0: none needed; host only), 0 for arguments that the call
- * refuses. Quantised rows live there, the partial sums of small products over long rows, and
+/* Workspace bytes of the call below (0: none needed; host only), 0 for a layer, type or number of
+ * rows that the call refuses. Quantised rows live there, the partial sums of small products over long rows, and
  * the copies of operands of large products that are not at 16-byte addresses and strides: the
  * weights' are known from the layer (a null weight counts as not), codes x as if they were not
  * (the call itself then needs less). It is the size for this number of rows: fewer rows may

@@ -113,6 +113,18 @@ def test_linear_takes_the_workspace_it_asks_for(fake, native):
         assert b"workspace" not in lib.fsx_last_error(ctx), (rows, k, n, xt, ldx, ldw, at, lib.fsx_last_error(ctx))
 
 
+def test_linear_workspace_of_refused_layers(fake, native):
+    """No size for a layer that the call refuses, whatever is wrong with it."""
+    over = dict(k=1000, n=500, ldw=1000, ldx=1000, ldy=500, xt=0, xs=None, rows=100)
+    assert native.linear_q8_work(native.q8_linear(P, P, None, 1000, 500), native.DTYPE_F32, 100) > 0
+    for bad in (dict(act=3), dict(act=-1), dict(reserved=1), dict(ldw=999), dict(ldw=1 << 52)):
+        a = {**over, **bad}
+        layer = native.q8_linear(P, P, None, a["k"], a["n"], a["ldw"], a.get("act", 0))
+        layer.reserved = a.get("reserved", 0)
+        assert native.linear_q8_work(layer, native.DTYPE_F32, 100) == 0, bad
+        assert lin(fake, native, P, 1 << 40, **a) == -errno.EINVAL, bad
+
+
 @pytest.mark.parametrize("rows", [(1 << 36) - 16, 1 << 36, (1 << 36) + 16, 1 << 37, (1 << 40) - 16, 1 << 40])
 def test_linear_workspace_of_many_rows(fake, native, rows):
     """Row counts whose blocks pass 32 bits: the size is worked out, and a product over so many
