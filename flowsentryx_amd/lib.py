@@ -360,6 +360,8 @@ class FsxContext:
                     "fsx_stream_wait_batches")
 
     def set_stream(self, stream_handle: int | None):
+        """Run on a caller's stream from here on; None or 0 (torch's default stream has that handle):
+        on the context's own stream, which is in no order with the default one."""
         self._check(self._lib.fsx_set_stream(self._h, stream_handle or None), "fsx_set_stream")
 
     # -- verdict path

@@ -211,7 +211,10 @@ int fsx_open(fsx_ctx **out, const fsx_config *cfg);
 void fsx_close(fsx_ctx *ctx);
 const char *fsx_last_error(const fsx_ctx *ctx);
 
-/* Attach a caller-owned hipStream_t (NULL restores the context's own stream). */
+/* Attach a caller-owned hipStream_t (NULL restores the context's own stream). NULL is not the
+ * null stream: the context's own stream is non-blocking, so work on the null stream (torch's
+ * default stream, whose handle is 0) is in no order with it. A program whose buffers are made
+ * or read on the null stream attaches a stream of its own and orders the two with events. */
 int fsx_set_stream(fsx_ctx *ctx, void *hip_stream);
 /* Wait for enqueued device work and report deferred device-side errors. */
 int fsx_sync(fsx_ctx *ctx);
