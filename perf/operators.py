@@ -221,10 +221,40 @@ def _context():
     return _program["lib"], _program["ctx"], _program["stream"]
 
 
+def _ready(s, lib, stream):
+    """What a program does once for its buffers: the layer, the workspace, and the stream's order behind
+    what made them, whichever stream that was."""
+    case = s["case"]
+    if case["op"] == "linear":
+        w = s["weight"]
+        act = {"none": lib.ACT_NONE, "relu": lib.ACT_RELU, "sigmoid": lib.ACT_SIGMOID}[case["act"]]
+        s["layer"] = lib.q8_linear(w.data_ptr(), s["weight_scale"].data_ptr(),
+                                   s["bias"].data_ptr() if s["bias"] is not None else None,
+                                   w.shape[1], w.shape[0], w.stride(0), act)
+        size = lib.linear_q8_work(s["layer"], _dtype(lib)[case["x"]], s["x"].shape[0])
+    elif case["op"] == "logprobs":
+        size = lib.logprobs_work(s["logits"].shape[0], s["logits"].shape[1], case["top"])
+    if case["op"] != "quantize":
+        s["work"] = torch.empty(size, dtype=torch.uint8, device="cuda")
+    stream.wait_stream(torch.cuda.current_stream())
+    for t in s.values():
+        if isinstance(t, torch.Tensor):
+            t.record_stream(stream)
+    s["ready"] = True
+
+
+def _dtype(lib):
+    return {"f32": lib.DTYPE_F32, "f16": lib.DTYPE_F16, "bf16": lib.DTYPE_BF16, "i8": lib.DTYPE_I8}
+
+
 def _own(s):
+    """The call, asynchronous on the program's stream: who changes the state's buffers or reads the
+    outputs on another stream waits for it first, as torch.cuda.synchronize() does."""
     lib, ctx, stream = _context()
     case = s["case"]
-    dtype = {"f32": lib.DTYPE_F32, "f16": lib.DTYPE_F16, "bf16": lib.DTYPE_BF16, "i8": lib.DTYPE_I8}
+    dtype = _dtype(lib)
+    if "ready" not in s:
+        _ready(s, lib, stream)
     if case["op"] == "quantize":
         x, q = s["x"], s["codes"]
         ctx.quantize_rows_device(x.data_ptr(), dtype[case["x"]], x.shape[0], x.shape[1], x.stride(0),
@@ -232,22 +262,12 @@ def _own(s):
         with torch.cuda.stream(stream):
             return dict(values=torch.mul(q, s["scale"][:, None]), scale=s["scale"])
     if case["op"] == "linear":
-        x, w, y = s["x"], s["weight"], s["y"]
-        if "layer" not in s:
-            act = {"none": lib.ACT_NONE, "relu": lib.ACT_RELU, "sigmoid": lib.ACT_SIGMOID}[case["act"]]
-            s["layer"] = lib.q8_linear(w.data_ptr(), s["weight_scale"].data_ptr(),
-                                       s["bias"].data_ptr() if s["bias"] is not None else None,
-                                       w.shape[1], w.shape[0], w.stride(0), act)
-            s["work"] = torch.empty(lib.linear_q8_work(s["layer"], dtype[case["x"]], x.shape[0]), dtype=torch.uint8,
-                                    device="cuda")
+        x, y = s["x"], s["y"]
         ctx.linear_q8_device(s["layer"], x.data_ptr(), dtype[case["x"]], x.stride(0),
                              s["x_scale"].data_ptr() if s["x_scale"] is not None else None, x.shape[0],
                              y.data_ptr(), dtype[case["y"]], y.stride(0), s["work"].data_ptr(), s["work"].numel())
         return y
     x = s["logits"]
-    if "work" not in s:
-        s["work"] = torch.empty(lib.logprobs_work(x.shape[0], x.shape[1], case["top"]), dtype=torch.uint8,
-                                device="cuda")
     ctx.logprobs_device(x.data_ptr(), dtype[case["x"]], x.shape[0], x.shape[1], x.stride(0), s["target"].data_ptr(),
                         s["logprob"].data_ptr(), s["entropy"].data_ptr(), case["top"], s["top_id"].data_ptr(),
                         s["top_logprob"].data_ptr(), s["work"].data_ptr(), s["work"].numel())
