@@ -1,6 +1,7 @@
 """The usage that the documents show for heads of other sizes, run as it stands there: on the CPU
 against streams that only write down who waits for whom, on the GPU for its answers."""
 import contextlib
+import importlib.util
 import re
 import types
 from pathlib import Path
@@ -11,11 +12,12 @@ import torch
 
 import head_ref
 
+ROOT = Path(__file__).resolve().parents[1]
 CALLS = ("quantize_rows_device", "linear_q8_device", "logprobs_device")
 
 
 def usage():
-    text = (Path(__file__).resolve().parents[1] / "INTEGRATION.md").read_text()
+    text = (ROOT / "INTEGRATION.md").read_text()
     block, = re.findall(r"## 8\. Heads.*?```python\n(.*?)```", text, re.S)
     return compile(block, "usage", "exec")
 
@@ -73,6 +75,37 @@ def test_usage_waits(native, monkeypatch):
     assert all(log[i][1] == handle for i in calls)
     assert ("wait", handle, 0) in log[:calls[0]], "inputs"
     assert ("wait", 0, handle) in log[calls[-1]:], "answers"
+
+
+@pytest.mark.parametrize("op", ["quantize", "linear", "logprobs"])
+def test_measured_calls_wait(native, monkeypatch, op):
+    """The measured cases' program: its stream is behind whichever stream made the buffers before its
+    first call on them, and the allocator knows that it uses them."""
+    spec = importlib.util.spec_from_file_location("measured", ROOT / "perf" / "operators.py")
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    log = []
+    mine = types.SimpleNamespace(cuda_stream=1, wait_stream=lambda other: log.append(("wait", other)))
+    call = lambda name: lambda *_: log.append(("call", name))
+    m._program.update(lib=native, stream=mine, ctx=types.SimpleNamespace(**{n: call(n) for n in CALLS}))
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *size, device=None, **kw: empty(*size, **kw))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: "caller")
+    monkeypatch.setattr(torch.cuda, "stream", lambda stream: contextlib.nullcontext())
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, stream: log.append(("kept", t.data_ptr(), stream)))
+    f, i = torch.zeros(200, 100), torch.zeros(200, 100, dtype=torch.int8)
+    v, n = torch.zeros(200), torch.zeros(200, dtype=torch.int32)
+    s = dict(quantize=dict(x=f, codes=i, scale=v),
+             linear=dict(x=f, x_scale=None, weight=i, weight_scale=v, bias=None, y=torch.zeros(200, 200)),
+             logprobs=dict(logits=f, target=n, logprob=v, entropy=v, top_id=n, top_logprob=v))[op]
+    s["case"] = dict(op=op, x="f32", y="f32", act="none", top=1)
+    m._own(s)
+    m._own(s)
+    calls = [k for k, e in enumerate(log) if e[0] == "call"]
+    assert len(calls) == 2 and ("wait", "caller") in log[:calls[0]]
+    for t in s.values():
+        if isinstance(t, torch.Tensor):
+            assert ("kept", t.data_ptr(), mine) in log[:calls[0]]
 
 
 @pytest.mark.gpu
