@@ -536,23 +536,22 @@ __global__ __launch_bounds__(BN / WN * (BM / WM) * 64) void k_linear_tile(Linear
 // The parts' sums, four channels of a row a thread.
 __global__ __launch_bounds__(256) void k_linear_join(LinearArgs a, int yt, uint32_t parts, const int32_t *sums) {
     const uint32_t per = (a.n + 3) / 4;
-    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < a.rows * per; i += gridDim.x * 256ull) {
-        const uint64_t r = i / per;
-        const uint32_t c = (uint32_t)(i - r * per) * 4;
-        v4i sum = {0, 0, 0, 0};
+    const uint64_t i = blockIdx.x * 256ull + threadIdx.x, r = i / per;
+    if (r >= a.rows) return;
+    const uint32_t c = (uint32_t)(i - r * per) * 4;
+    v4i sum = {0, 0, 0, 0};
 #pragma unroll 8
-        for (uint32_t p = 0; p < parts; ++p) {
-            const int32_t *from = sums + (p * a.rows + r) * a.n + c;
+    for (uint32_t p = 0; p < parts; ++p) {
+        const int32_t *from = sums + (p * a.rows + r) * a.n + c;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] += from[c + e < a.n ? e : 0];
-        }
-        put_sums(a, yt, sum, a.x_scale[r], r, c);
+        for (int e = 0; e < 4; ++e) sum[e] += from[c + e < a.n ? e : 0];
     }
+    put_sums(a, yt, sum, a.x_scale[r], r, c);
 }
 
 static void join_parts(const LinearArgs &a, int yt, uint32_t parts, const int32_t *sums, hipStream_t st) {
-    const uint64_t blocks = (a.rows * ((a.n + 3) / 4) + 255) / 256;
-    k_linear_join<<<(uint32_t)std::min<uint64_t>(blocks, 4096), 256, 0, st>>>(a, yt, parts, sums);
+    const uint64_t blocks = (a.rows * ((a.n + 3) / 4) + 255) / 256;   // (products in parts: a few thousand at most)
+    k_linear_join<<<(uint32_t)blocks, 256, 0, st>>>(a, yt, parts, sums);
 }
 
 // Rows that the DMA cannot bring into rows that it can, 16 bytes a thread; 0 behind their ends.

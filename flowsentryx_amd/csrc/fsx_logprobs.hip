@@ -700,52 +700,50 @@ __global__ __launch_bounds__(64 * W, 8) void k_logprobs_long(LogprobArgs a, uint
     }
 }
 
-// The parts of a row: a lane of the first wave takes a part's sums; the waves take the parts'
-// alternatives in turn, above a lower bound from the first few of every part.
+// The parts of a row, a block for each: a lane of the first wave takes a part's sums; the waves take
+// the parts' alternatives in turn, above a lower bound from the first few of every part.
 template <int DT, bool TOP>
 __global__ __launch_bounds__(256) void k_logprobs_join(LogprobArgs a, uint32_t parts) {
     constexpr int W = 4;
     __shared__ Shared<W> sh;
     const uint32_t lane = __lane_id(), wave = wave_id();
-    for (uint64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        Sums q;
-        Pool pool{sh.pool[wave], 0};
-        q.init();
-        int32_t t = -1;
-        float xt = 0.0f;
-        if (threadIdx.x == 0) given<DT>(a, r, t, xt);
-        if (TOP) {
-            const uint32_t per = (a.top > kFewTop ? 256 : 64) / parts, nth = threadIdx.x / parts;
-            const Alt sample = nth < a.top && nth < per ? Part(a, r * parts + threadIdx.x % parts).alts[nth] : 0;
-            __syncthreads();   // (the row before still reads the words)
-            if (threadIdx.x == 0) sh.total = 0;
-            sh.word[threadIdx.x] = (uint32_t)(sample >> 32);
-        }
-        if (wave == 0 && lane < parts) {
-            const Part from(a, r * parts + lane);
-            q.join(from.sums[0], from.sums[1], from.sums[2]);
-        }
-        q.template join_group<64>();
-        if (TOP) {
-            __syncthreads();
-            const uint32_t low = bound(sh, a.top);
+    const uint64_t r = blockIdx.x;
+    Sums q;
+    Pool pool{sh.pool[wave], 0};
+    q.init();
+    int32_t t = -1;
+    float xt = 0.0f;
+    if (threadIdx.x == 0) given<DT>(a, r, t, xt);
+    if (TOP) {
+        const uint32_t per = (a.top > kFewTop ? 256 : 64) / parts, nth = threadIdx.x / parts;
+        const Alt sample = nth < a.top && nth < per ? Part(a, r * parts + threadIdx.x % parts).alts[nth] : 0;
+        if (threadIdx.x == 0) sh.total = 0;
+        sh.word[threadIdx.x] = (uint32_t)(sample >> 32);
+    }
+    if (wave == 0 && lane < parts) {
+        const Part from(a, r * parts + lane);
+        q.join(from.sums[0], from.sums[1], from.sums[2]);
+    }
+    q.template join_group<64>();
+    if (TOP) {
+        __syncthreads();
+        const uint32_t low = bound(sh, a.top);
 #pragma unroll 1
-            for (uint32_t p = wave; p < parts; p += 4 * W) {
-                Alt mine[4];
+        for (uint32_t p = wave; p < parts; p += 4 * W) {
+            Alt mine[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    mine[j] = p + j * W < parts && lane < a.top ? Part(a, r * parts + p + j * W).alts[lane] : 0;
+            for (int j = 0; j < 4; ++j)
+                mine[j] = p + j * W < parts && lane < a.top ? Part(a, r * parts + p + j * W).alts[lane] : 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (pool.n + 64 > kPool) pool.keep_best(a.top);
-                    const bool want = mine[j] != 0 && (uint32_t)(mine[j] >> 32) >= low;
-                    pool.put(__ballot(want), want, mine[j]);
-                }
+            for (int j = 0; j < 4; ++j) {
+                if (pool.n + 64 > kPool) pool.keep_best(a.top);
+                const bool want = mine[j] != 0 && (uint32_t)(mine[j] >> 32) >= low;
+                pool.put(__ballot(want), want, mine[j]);
             }
         }
-        const Alt alt = block_join<W, TOP>(sh, q, pool, a.top);
-        if (wave == 0) finish_row(a, r, q, alt, t, xt);
     }
+    const Alt alt = block_join<W, TOP>(sh, q, pool, a.top);
+    if (wave == 0) finish_row(a, r, q, alt, t, xt);
 }
 
 // Many rows: a block of four waves each. Fewer: of sixteen, each with less to do, and with
@@ -769,7 +767,7 @@ static void logprobs(const LogprobArgs &a, hipStream_t st) {
     else if (a.rows >= kManyRows && a.v <= 4096) k_logprobs_long<DT, 4, 2, TOP><<<grid, 64 * 4, 0, st>>>(a, 1);
     else if (a.rows >= kManyRows) k_logprobs_long<DT, 4, 4, TOP><<<grid, 64 * 4, 0, st>>>(a, 1);
     else k_logprobs_long<DT, kFewW, kFewH, TOP><<<grid, 64 * kFewW, 0, st>>>(a, parts);
-    if (parts > 1) k_logprobs_join<DT, TOP><<<(uint32_t)std::min<uint64_t>(a.rows, 1u << 16), 256, 0, st>>>(a, parts);
+    if (parts > 1) k_logprobs_join<DT, TOP><<<(uint32_t)a.rows, 256, 0, st>>>(a, parts);   // (up to 170 rows)
 }
 
 uint64_t logprobs_work(uint64_t rows, uint32_t v, uint32_t top) {

@@ -152,6 +152,21 @@ def test_logprobs_refusals(fake, over, word):
     refused(fake, logp(fake, **over), word)
 
 
+def test_parts_are_few(fake, native):
+    """A call in parts has another launch that joins them, a block for a row and a thread for four
+    channels: rows and products that are cut are small enough for one."""
+    for classes in (8193, 70001, 131072, (1 << 31) - 1):
+        for rows in list(range(1, 1100)) + [1 << 16, 1 << 36, 1 << 40]:
+            assert (native.logprobs_work(rows, classes, 5) > 0) == (rows <= 170), (rows, classes)
+    rng = random.Random(6)
+    for _ in range(20000):
+        rows, k, n = (int(2 ** rng.uniform(0, top)) for top in (41, 17, 31))
+        layer = native.q8_linear(P, P, None, min(k, 131071), n, min(k, 131071) + 15 & ~15)
+        copies = rows * int(layer.ld_weight) if rows * k * n >= 2.5e9 and n >= 384 else 0
+        sums = native.linear_q8_work(layer, native.DTYPE_I8, min(rows, 1 << 40)) - copies
+        assert sums <= 64 * 4 * (1 << 20) + 16, (rows, k, n)   # (parts, bytes, results)
+
+
 def test_nothing_to_do_is_no_error(fake, native):
     assert quant(fake, rows=0) == 0
     assert lin(fake, native, rows=0) == 0
