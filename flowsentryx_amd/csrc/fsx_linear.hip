@@ -1,8 +1,9 @@
-// fsx_linear.hip — int8 layers of free size: the row quantiser and the int8 matrix product
-// with a scale for every row of x and every output channel (include/fsx_hip.h).
+// fsx_linear.hip — int8 layers of free size (include/fsx_hip.h fsx_linear_q8_device): the int8
+// matrix product with a scale for every row of x and every output channel,
 //
-//   scale_r = max(fl32(max_c |x_rc| / 127), 2^-126)      q_rc = rhe(x_rc / scale_r)
-//   y_rn    = act((float)(sum_k q_rk w_nk) * scale_r * t_n + b_n)
+//   y_rn = act((float)(sum_k q_rk w_nk) * scale_r * t_n + b_n)
+//
+// and which kernel takes it. Floats become codes q as fsx_quantize.hip makes them.
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <type_traits>
