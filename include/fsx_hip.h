@@ -305,10 +305,14 @@ int fsx_score_device(fsx_ctx *ctx, const float *d_features, size_t n, float *d_p
  *
  * All buffers are device memory of the context's GPU, rows are `ld` elements apart (ld >= the
  * row's length; a row's end up to ld is neither read as data nor written), and outputs do not
- * overlap inputs, each other or the workspace. The calls are asynchronous on the context
- * stream and keep nothing: no device memory is allocated, nothing is cached between calls, so
- * they may be captured into a HIP graph (a workspace is then the graph's own: one that two
- * graphs share is overwritten when both run at once). With 0 rows nothing is launched.
+ * overlap inputs, each other or the workspace. Codes are loaded in whole words at multiples of 4
+ * or 16 bytes: the words that a buffer's first and last codes lie in are read whole (up to 3
+ * bytes before it and 15 behind it), and what is not the buffer's does not count. The calls are
+ * asynchronous on the context stream and keep nothing: no device memory is allocated, nothing is
+ * cached between calls, so they may be captured into a HIP graph (a workspace is then the graph's
+ * own: one that two graphs share is overwritten when both run at once; a capture begins with no
+ * pipelined batch under way, fsx_sync before it, since the captured stream would wait for work
+ * outside the graph). With 0 rows nothing is launched.
  * Results do not depend on timing: the same call gives the same bits.
  *
  * Errors: -EINVAL (with fsx_last_error) for an unknown type, a null or misaligned pointer
