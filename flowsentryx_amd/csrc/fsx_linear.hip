@@ -591,14 +591,27 @@ static bool dma_can(const void *p, uint64_t ld) { return ((uintptr_t)p | ld) % 1
 // and 28.2 / 28.4). Few channels, 2^20 rows of 1024 to 16: 277, in tiles 317.
 // kTiles: k_linear_tile.
 //
-// Few blocks over a long k are cut into parts; the join is another launch. In tiles: 40 rows of
-// 10931 to 42 channels 14.3 us in 10 parts, 13.3 in 20; through registers more tiles are cut (107
-// rows of 6581 to 6892 channels 57 -> 38) than by DMA (603 rows of 3982 to 1394 22.6 -> 25.9: not).
-// Direct: 14 rows of 11313 to 1384 channels 24 -> 12.8, but one row of 4096 to 1024 channels 4.8 ->
-// 7.1: by the bytes that a block takes.
-// Operands that the DMA cannot bring are packed for it where the work repays the copy: 4096 rows
-// of 4096 to 4096 channels at odd strides 182 -> 78 us, 1006 rows of 8444 to 2643 channels 104 ->
-// 64, but 1000 rows of 1003 to 777 channels 8.0 -> 12.2.
+// Few blocks over a long k are cut into parts; the join is another launch (us of codes, whole and
+// in parts).
+//   Tiles by DMA: 40 rows of 4096 / 8192 / 32768 to 64 channels 8.9 / 14.9 / 78 and 8.5 / 11.1 / 27, 300
+//     rows of 8192 / 16384 to 1024 23 / 41 and 18 / 21, but of 2048 / 4096 6.4 / 13.0 and 13.7 / 16.9:
+//     with some 80 tiles and more the rule cuts before it pays. 128 tiles and more are not cut (603 rows of
+//     3984 to 1394 15.5 and 19.1).
+//   Tiles through registers: 100 rows of 1024 / 2048 / 4096 to 500 8.1 / 13.2 / 23.6 and 9.4 / 10.2 /
+//     11.8; up to 256 tiles from 4096 on: 107 rows of 6581 to 6892 56 and 38, 900 of 4096 / 8192 to 900
+//     24.8 / 37.5 and 28.4 / 34.3.
+//   Direct, by the bytes that a block takes (400000: up to 16 rows a k of 12500, up to 32 of 8334, half of
+//     it at odd strides): to 1024 channels one row of 4096 / 8192 / 12544 4.8 / 7.7 / 10.5 and 8.2 / 7.5 /
+//     8.4, 14 rows of 4096 / 8192 / 12544 6.0 / 9.3 / 12.8 and 7.1 / 8.3 / 9.6, 30 rows of 4096 / 8448
+//     7.7 / 13.1 and 8.2 / 9.8, 14 rows at odd strides of 4096 / 6300 7.7 / 10.2 and 7.8 / 8.7; 1000 rows
+//     of 8192 / 12544 to 12 9.0 / 12.5 and 8.3 / 9.7.
+// Operands that the DMA cannot bring are packed for it where the work repays the copy (us, as they
+// are and packed): 4096 rows of 4096 to 4096 channels at odd strides 182 and 78, 1006 rows of 8444 to
+// 2643 104 and 64; odd weights and bf16 rows of 4096 to 4096, 128 / 200 / 300 / 384 / 512 / 768 rows 24.5 /
+// 34.3 / 37.3 / 38.0 / 38.9 / 43.2 and 28.7 / 29.9 / 32.3 / 32.0 / 31.1 / 37.3; odd codes of 4096 rows, 128 /
+// 384 / 512 / 768 channels 19.5 / 27.0 / 27.4 / 32.8 and 25.0 / 26.1 / 25.4 / 35.3. About the least work packed it
+// goes by k: 700 rows of 2000 to 2000 24.0 and 22.2, 2000 of 1000 to 2000 20.8 and 21.7, 1000 of 1003 to 2500
+// 17.4 and 20.8 (both odd, codes: 11.0 and 18.4).
 enum LinearForm { kNarrow, kDirectFloats, kDirect, kTiles };
 struct LinearPlan {
     LinearForm form;
@@ -660,6 +673,9 @@ struct LinearPlan {
 //   128 x 128, two buffers           26    28    37    71-77 (572)
 //   128 x 128, four buffers          23    25    55    95    (one block a CU)
 //    64 x 64                         16    33    64   119    (909)
+// Between, at 640 / 768 / 896 / 1152 rows (160 / 192 / 224 / 288 tiles of 128), 128 x 128 with four buffers and
+// 64 x 64: 22.6 / 22.7 / 23.2 / 43.1 and 26.3 / 26.5 / 27.5 / 38.6, over a k of 1024 9.9 / 10.3 / 10.6 / 18.8 and
+// 10.4 / 10.7 / 11.7 / 15.3.
 // Over a short k what a tile loads and stores first and last counts, and 256 x 256 with one block a CU
 // has nothing beside it: 8192 rows of 256 / 2048 to 8192 channels 119 / 215 us, 128 x 128 81 / 200. Up
 // to 64 channels larger tiles multiply zeros: 100000 rows of 256 to 64 24 us, 128 x 128 14.0, 64 x 64

@@ -377,10 +377,12 @@ template <int DT, int N, int G> static bool logprobs_short(const LogprobArgs &a,
     const uint32_t grid = (uint32_t)std::min<uint64_t>(blocks, 256 * 8);   // (the blocks that fit at once)
     const uint32_t top_inv = a.top ? ((1u << 18) + a.top - 1) / a.top : 0;
     // A few alternatives: kept in registers and stored as they come (us of 2^22 rows of 16 f32 logits,
-    // 1 / 3 / 5 alternatives: 84 / 110 / 145, by way of LDS 93 / 114 / 147; 200000 rows of 33, 3 / 5 / 8: 26 /
-    // 34 / 45 and 26 / 31 / 38). Counting costs what the row is long, choosing what is asked for: about
-    // v (2 N + 2) and 3 / 5 top (4 N + 3 log2 G + 14) instructions a lane (33 classes: counting 51 us, choosing
-    // 18 + 2.4 top; 2^20 rows of 7 f16 logits, 28 asked for: 64 us, where one by one took 376).
+    // 1 / 3 / 5 alternatives: 72 / 88 / 112, by way of LDS 77 / 92 / 115; 200000 bf16 rows of 200, 1 / 3 / 4 / 8:
+    // 45 / 64 / 74 / 113 and 51 / 65 / 72 / 102). Counting costs what the row is long, choosing what is asked
+    // for: about v (2 N + 2) and 3 / 5 top (4 N + 3 log2 G + 14) instructions a lane (us, counted and one by one: 2^19
+    // rows of 16, 8 / 12 / 16 asked for 24 / 26 / 27 and 22 / 27 / 33; 2^18 of 33, 12 / 20 / 33 63 / 65 / 69 and 47 /
+    // 67 / 101; 2^18 of 64, 24 / 32 / 48 89 / 90 / 93 and 74 / 93 / 132; 2^17 of 100, 32 / 48 / 64 124 / 125 / 128 and 96 /
+    // 136 / 176; of 128, always one by one, 48 / 64 150 / 151 and 131 / 170).
     constexpr uint32_t log_g = G > 32 ? 6 : G > 16 ? 5 : G > 8 ? 4 : G > 4 ? 3 : G > 2 ? 2 : G > 1 ? 1 : 0;
     const uint32_t rank_cost = G == 1 ? 2 * N * N : a.v * (2 * N + 2),
                    rounds_cost = std::min(a.top, a.v) * (4 * N + 3 * log_g + 14);
@@ -398,8 +400,9 @@ template <int DT, int N, int G> static bool logprobs_short(const LogprobArgs &a,
         }
     }
     // Bounding costs the same for any number, if there are lanes enough for a bound (us of 20000 bf16 rows of
-    // 500, 5 / 12 / 20 asked for: bounded 21.5 / 22.9 / 24.6, chosen 22.7 / 33.3 / 46.8; of 200, half a wave a row: 11.9 /
-    // 13.4 / 17.5 and 10.3 / 15.2 / 20.9, with 24 of 25 lanes 28.0 and 23.9; a quarter of a wave gains nothing).
+    // 500, 4 / 12 / 40 / 56 asked for: bounded 16.5 / 18.6 / 26 / 91, chosen 17.8 / 31 / 79 / 108; of 200, half a wave a row,
+    // 5 / 9 / 20 / 22: 11.6 / 12.6 / 17.1 / 22.1 and 9.9 / 12.9 / 21.1 / 22.6, with 24 of 25 lanes 28.7 and 24.0; a
+    // quarter of a wave gains nothing).
     if constexpr (G >= 32) {
         if (a.top >= (G == 64 ? 4 : 9) && 8 * ((a.v + N - 1) / N) >= 9 * a.top) {
             if (a.v % N == 0) go(k_logprobs_short<DT, N, G, true, kBound>);
@@ -412,9 +415,9 @@ template <int DT, int N, int G> static bool logprobs_short(const LogprobArgs &a,
     return true;
 }
 // Eight logits a lane as far as 64 lanes reach, then sixteen, unless more alternatives are asked for than
-// its lanes can bound; else in blocks (20000 bf16 rows of 1004, 1 / 5 / 20 alternatives 19 / 27 / 30 us, in
-// blocks 40 / 43 / 49; 40 of 600, one by one: 127 and 63). 32 a lane leave too few waves (31582 rows of 1279, 1 / 5 / 20:
-// 48 / 86 / 95, in blocks 62 / 68 / 78).
+// its lanes can bound; else in blocks (20000 bf16 rows of 1004, 0 / 1 / 5 / 20 / 40 alternatives 12.3 / 17.7 / 27 / 31 / 38
+// us, in blocks 20 / 40 / 44 / 49 / 62; 40 of 600, one by one: 127 and 63). 32 a lane leave too few waves (31582 rows of
+// 1279, 1 / 5 / 20: 48 / 86 / 95, in blocks 63 / 70 / 79).
 constexpr uint32_t kShort = 64 * 8;
 constexpr uint64_t kManyRows = 1024;   // for long rows: blocks of four waves from here on
 constexpr uint32_t kPool = 128;       // a wave's candidates: 64 alternatives and one of every lane
@@ -424,8 +427,10 @@ template <int DT> static bool logprobs_short(const LogprobArgs &a, hipStream_t s
         if (a.v > 1024 || (a.top > 3 && 8 * ((a.v + 15) / 16) < 9 * a.top)) return false;
         return logprobs_short<DT, 16, 64>(a, st);
     }
-    // 32-bit logits four a lane where half the lanes would do nothing, or where a bound needs more of them
-    // (2^22 rows of 16, 1 / 3 alternatives: 93 / 114 us, eight a lane 76 / 98; 50000 of 200, 3 / 30: 29 / 42 and 18 / 70)
+    // 32-bit logits four a lane where half the lanes would do nothing, or where a bound needs more of them (us,
+    // four and eight a lane: 2^22 rows of 16, 1 / 3 alternatives 79 / 107 and 71 / 87; 100000 of 175, 6 / 9 / 12 / 15 / 18 /
+    // 30 56 / 59 / 61 / 64 / 67 / 85 and 50 / 58 / 62 / 67 / 75 / 148, of 256, 9 / 15 / 26 / 40 60 / 66 / 76 / 96 and 59 / 66 /
+    // 100 / 173; of 140 with 40, which the lanes of neither can bound, 267 and 191)
     if constexpr (DT == FSX_DTYPE_F32) {
         if (a.v <= 4) return logprobs_short<DT, 4, 1>(a, st);
         if (a.v > 128 && a.v <= 256 && a.top > 8) return logprobs_short<DT, 4, 64>(a, st);
@@ -759,10 +764,10 @@ template <int DT, bool TOP>
 static void logprobs(const LogprobArgs &a, hipStream_t st) {
     const uint32_t parts = long_parts(a.rows, a.v);
     const dim3 grid(parts, (uint32_t)std::min<uint64_t>(a.rows, 65535));
-    // Pieces as large as all waves of a block have some: 20000 rows of 2048 with 1 / 20 / 64 alternatives 41 /
-    // 52 / 75 us with pieces of 512, 47 / 68 / 950 with 2048; 9183 rows of 3199, 20 alternatives, pieces of
-    // 512 / 1024 / 2048: 38 / 32 / 39; 10000 of 5000: 50 / 50 / 45. 700 rows of 2048: 5.5 - 8.2 us, with sixteen waves
-    // a row 8.6 - 12.8.
+    // Pieces as large as all waves of a block have some (us, pieces of 512 / 1024 / 2048): 20000 rows of 2048 with
+    // 1 / 20 / 64 alternatives 42 / 43 / 47, 53 / 57 / 68, 78 / 87 / 950; 31582 of 1279 with 5 70 / 77 / 90; 9183 of
+    // 3199 with 20 39 / 32 / 38; 10000 of 5000 52 / 49 / 44. 700 rows of 2048: 5.5 - 8.2 us, with sixteen waves a row
+    // 8.6 - 12.8.
     if (a.v <= 2048) k_logprobs_long<DT, 4, 1, TOP><<<grid, 64 * 4, 0, st>>>(a, 1);
     else if (a.rows >= kManyRows && a.v <= 4096) k_logprobs_long<DT, 4, 2, TOP><<<grid, 64 * 4, 0, st>>>(a, 1);
     else if (a.rows >= kManyRows) k_logprobs_long<DT, 4, 4, TOP><<<grid, 64 * 4, 0, st>>>(a, 1);
